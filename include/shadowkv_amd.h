@@ -589,6 +589,55 @@ int skv_linear_qkv_rope_append(const uint16_t* x, int64_t x_stride, const uint16
                                int64_t kv_stride_b, int64_t kv_stride_h, int64_t kv_stride_s,
                                const int64_t* append_row, int64_t buf_len, void* stream);
 
+/* ---- 8-bit KV cache ------------------------------------------------------------------------
+ * No reference counterpart: the reference's caches are bf16 throughout. A cache of keys or values is
+ * e4m3 codes (OCP, "fn") and an fp32 scale per block of `block` (16, 32, 64 or 128) tokens and head;
+ * a value is code * scale. Code row s of (b, h): codes + b*c_stride_b + h*c_stride_h + s*c_stride_s (bytes,
+ * multiples of 16; 128 bytes, 16-byte aligned), s < cap; scale of block j: scale + b*s_stride_b +
+ * h*s_stride_h + j (fp32, not negative). Keys and values share the strides.
+ *
+ * skv_kv8_write: rows t < n_b of k and v (bf16 rows of 128 at base + b*stride_b + h*stride_h + t*stride_t,
+ * multiples of 8 elements, 16-byte aligned) into positions start[b] + t < cap, n_b = counts[b] clamped to [0,
+ * rows] (counts null: rows); start and counts on the device; a sequence with start[b] < 0 is left alone.
+ * In each block with a new row, need = the smallest power of two, at least 2^-126, under which the new
+ * rows' largest finite magnitude is at most 448; the block's scale becomes need, or, where it holds older rows (of
+ * its positions before start[b]), max(scale, need), and those are encoded again where that is larger.
+ * Codes are value / scale to nearest even; infinities and NaN become NaN (the format has no infinity).
+ * Every other code and scale stays as it is. The results do not depend on the order of execution. */
+int skv_kv8_write(const uint16_t* k, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, const uint16_t* v,
+                  int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, uint8_t* k8, uint8_t* v8,
+                  int64_t c_stride_b, int64_t c_stride_h, int64_t c_stride_s, float* k_scale, float* v_scale,
+                  int64_t s_stride_b, int64_t s_stride_h, const int32_t* start, const int32_t* counts, int batch_size,
+                  int heads, int rows, int cap, int block, void* stream);
+
+/* Rows of one cache (keys or values) as bf16: out [batch, heads, rows, 128] (contiguous, 16-byte aligned) =
+ * bf16(code * scale), exact for scales that are powers of two and values in bf16's normal range. chunk_ids null:
+ * rows start to start + rows - 1. Else (start 0) [batch, heads, rows / chunk_size] ids (int64), row i*chunk_size + j
+ * of out being row chunk_ids[i]*chunk_size + j of the cache; rows outside [0, cap) read as zeros. codes may be the
+ * device address of pinned host memory. */
+int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_stride_h, int64_t c_stride_s, const float* scale,
+                 int64_t s_stride_b, int64_t s_stride_h, const int64_t* chunk_ids, int chunk_size, int64_t start,
+                 uint16_t* out, int batch_size, int heads, int rows, int cap, int block, void* stream);
+
+/* Attention of new tokens over such a cache: query t < n_b (n_b as above, from counts) of sequence b is at position
+ * p = length_b - n_b + t, length_b = lengths[b] clamped to [0, cap], and sees the keys j <= p, with a
+ * window > 0 only those with j > p - window or j < sinks:
+ *   out[b, t, hq, :] = sum_j exp(scale q[b, hq, t] . k_j) v_j / sum_j exp(scale q[b, hq, t] . k_j)
+ * over them, of kv head hq / (q_heads / kv_heads); zeros for a query that sees nothing (p < 0) and for t >= n_b.
+ * Keys and values that a query does not see do not reach it, whatever they hold. Scores, probabilities and sums
+ * in fp32, out [batch, rows, q_heads, 128] bf16 (contiguous, 16-byte aligned). q: rows of 128 bf16 at
+ * q + b*q_stride_b + hq*q_stride_h + t*q_stride_t, multiples of 8 elements, 16-byte aligned. lengths and counts
+ * are read when the kernels run. workspace: skv_kv8_attn_workspace_bytes bytes (0 for some sizes, and for bad
+ * ones), 16-byte aligned, overwritten. */
+int64_t skv_kv8_attn_workspace_bytes(int batch_size, int q_heads, int kv_heads, int rows, int cap, int window,
+                                     int sinks);
+int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, const uint8_t* k8,
+                 const uint8_t* v8, int64_t c_stride_b, int64_t c_stride_h, int64_t c_stride_s, const float* k_scale,
+                 const float* v_scale, int64_t s_stride_b, int64_t s_stride_h, const int32_t* lengths,
+                 const int32_t* counts, int batch_size, int q_heads, int kv_heads, int rows, int cap, int block,
+                 float scale, int window, int sinks, uint16_t* out, void* workspace, int64_t workspace_bytes,
+                 void* stream);
+
 /* ---- measurement -------------------------------------------------------------------------
  * HBM read envelope probe. No reference counterpart: it measures what a read-only launch of a
  * given size reaches, the ceiling the streaming kernels are read against. Reads `tiles` tiles of

@@ -108,6 +108,13 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "skv_fetch_misses_rebuild_k_rope": (
         _i32, [_p, _p, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _i64, _i64, _p, _p,
                _i64, _i64, _i32, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _i32, _p]),
+    "skv_kv8_write": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64,
+                             _p, _p, _i32, _i32, _i32, _i32, _i32, _p]),
+    "skv_kv8_read": (_i32, [_p, _i64, _i64, _i64, _p, _i64, _i64, _p, _i32, _i64, _p, _i32, _i32, _i32, _i32, _i32,
+                            _p]),
+    "skv_kv8_attn_workspace_bytes": (_i64, [_i32, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "skv_kv8_attn": (_i32, [_p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _p, _p, _i32, _i32,
+                            _i32, _i32, _i32, _i32, _f32, _i32, _i32, _p, _p, _i64, _p]),
     "skv_hbm_read_probe": (_i32, [_p, _i64, _i32, _i32, _p, _i64, _p]),
     "skv_mfma_peak_probe": (_i32, [_i32, _i32, _p, _i64, _p]),
     "skv_mfma_peak_probe_flops": (_i64, [_i32, _i32]),

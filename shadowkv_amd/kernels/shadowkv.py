@@ -29,7 +29,7 @@ __all__ = [
     "apply_rotary_pos_emb_new", "apply_rotary_pos_emb_push_cache_opt", "apply_rotary_pos_emb_push_cache_opt_glm",
     "batch_gather_gemm", "batch_gemm_softmax", "score_gqa_max", "score_logits", "softmax_gqa_max", "select_chunks", "topk_gather", "rebuild_k_rope",
     "sparse_attn_workspace_bytes", "sparse_attn_workspace", "sparse_attn_decode", "sparse_attn_xcd_check",
-    "device_address", "select_workspace_bytes",
+    "device_address", "select_workspace_bytes", "kv8_write", "kv8_read", "kv8_read_chunks", "kv8_attn",
 ]
 
 
@@ -1170,6 +1170,170 @@ def gather_copy_misses_to_slots(values, v_cache_buffer, miss_ids, cnts, miss_slo
     _lib.call("skv_gather_copy_misses_to_slots", device_address(values), v_cache_buffer.data_ptr(), miss_ids.data_ptr(),
               cnts.data_ptr(), miss_slot.data_ptr(), batch_size, heads, row_stride, pool_offset, gpu_v_stride,
               map_size, pool_slots, chunk_elems, _stream())
+
+
+# ---------------------------------------------------------------------------------------------
+# 8-bit KV cache: codes e4m3 [B, H, cap, 128] and fp32 scales [B, H, >= ceil(cap / block)], a value is code * scale
+
+KV8_BLOCKS = (16, 32, 64, 128)
+KV8_MAX_TOKENS = 2 ** 30
+
+
+def _no_grad(what: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
+
+
+def _rows128(t: torch.Tensor, name: str) -> torch.Tensor:
+    """t [B, heads, rows, 128] bf16 as it is where its rows can be read 16 bytes at a time, else a copy."""
+    _dev(t, name, torch.bfloat16)
+    if t.dim() != 4 or t.shape[3] != 128 or t.numel() == 0:
+        raise ValueError(f"{name} {tuple(t.shape)} must be [B, heads, rows, 128], none of them empty")
+    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in _strides(t, 3))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides(t: torch.Tensor, n: int) -> tuple:
+    """The first n strides of t, those of axes with one entry as 0 (torch leaves them open)."""
+    return tuple(st if sz > 1 else 0 for st, sz in zip(t.stride()[:n], t.shape))
+
+
+def _kv8_ints(t: torch.Tensor, name: str, B: int, device) -> int:
+    _dev(t, name, torch.int32)
+    if t.shape != (B,) or not t.is_contiguous() or t.device != device:
+        raise ValueError(f"{name} must be {B} contiguous int32 on {device}, got {tuple(t.shape)} on {t.device}")
+    return t.data_ptr()
+
+
+def _kv8_cache(codes: torch.Tensor, scale: torch.Tensor, name: str, block: int, device=None):
+    """Checks one cache; returns (B, H, cap)."""
+    if block not in KV8_BLOCKS:
+        raise ValueError(f"block={block} must be one of {KV8_BLOCKS}")
+    _dev(scale, f"{name} scale", torch.float32)
+    if codes.dtype != torch.float8_e4m3fn:
+        raise ValueError(f"{name} must be torch.float8_e4m3fn, got {codes.dtype}")
+    if codes.dim() != 4 or codes.shape[3] != 128 or codes.numel() == 0 or codes.stride(3) != 1 or \
+            codes.data_ptr() % 16 or any(s % 16 for s in _strides(codes, 3)):
+        raise ValueError(f"{name} {tuple(codes.shape)} must be [B, H, capacity, 128] with contiguous rows, 16-byte "
+                         "aligned (strides multiples of 16)")
+    B, H, cap, _ = codes.shape
+    if cap > KV8_MAX_TOKENS:
+        raise ValueError(f"{name} holds {cap} tokens (at most {KV8_MAX_TOKENS})")
+    if scale.dim() != 3 or scale.shape[:2] != (B, H) or scale.shape[2] < (cap + block - 1) // block or \
+            scale.stride(2) != 1:
+        raise ValueError(f"{name} scale {tuple(scale.shape)} must be [{B}, {H}, {(cap + block - 1) // block} or more] "
+                         "with contiguous rows")
+    if scale.device != (codes.device if device is None else device):
+        raise ValueError(f"{name} and its scale must be on one device")
+    return B, H, cap
+
+
+def _kv8_pair(k8, v8, k_scale, v_scale, block):
+    """Checks keys and values of one layout; returns (B, H, cap)."""
+    _dev(k8, "k8"), _dev(v8, "v8")
+    geo = _kv8_cache(k8, k_scale, "k8", block)
+    _kv8_cache(v8, v_scale, "v8", block)
+    if k8.shape != v8.shape or _strides(k8, 3) != _strides(v8, 3) or \
+            _strides(k_scale, 2) != _strides(v_scale, 2) or k8.device != v8.device:
+        raise ValueError("k8 and v8 (and their scales) must share a layout and a device")
+    return geo
+
+
+def _distinct(t: torch.Tensor) -> bool:
+    """Whether no two elements of t can share memory."""
+    extent = 1
+    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+        if stride < extent:
+            return False
+        extent += (size - 1) * stride
+    return True
+
+
+def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
+    """New tokens' keys and values into an 8-bit cache, in place: rows t < counts[b] (all, without counts) of
+    k, v [B, H, T, 128] (bf16, any strides) become the positions start[b] + t of k8, v8 [B, H, capacity, 128]
+    (float8_e4m3fn); those at the capacity and behind are dropped, and a sequence with start[b] < 0 is left alone.
+    start, counts: device int32 [B], read when the kernel runs.
+    A block's scale is the smallest power of two under which its new rows fit; where it holds older rows (before
+    start[b]) it never falls, and they are encoded again where it grows. Infinities become NaN. Nothing else in
+    the caches changes."""
+    B, H, cap = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    _no_grad("kv8_write", k, v)
+    k, v = _rows128(k, "k"), _rows128(v, "v")
+    if k.shape != v.shape or k.shape[:2] != (B, H):
+        raise ValueError(f"kv8_write: k {tuple(k.shape)} v {tuple(v.shape)} for caches of [{B}, {H}]")
+    if k.device != k8.device or v.device != k8.device:
+        raise ValueError("kv8_write: rows and caches must be on one device")
+    if not all(_distinct(t) for t in (k8, v8, k_scale, v_scale)) or k8.data_ptr() == v8.data_ptr() or \
+            k_scale.data_ptr() == v_scale.data_ptr():
+        raise ValueError("kv8_write: the caches must not share memory with themselves or each other")
+    sp = _kv8_ints(start, "start", B, k8.device)
+    cp = None if counts is None else _kv8_ints(counts, "counts", B, k8.device)
+    with torch.cuda.device(k8.device):
+        _lib.call("skv_kv8_write", k.data_ptr(), *_strides(k, 3), v.data_ptr(), *_strides(v, 3), k8.data_ptr(),
+                  v8.data_ptr(), *_strides(k8, 3), k_scale.data_ptr(), v_scale.data_ptr(), *_strides(k_scale, 2), sp, cp,
+                  B, H, k.shape[2], cap, block, _stream())
+
+
+def _kv8_read(codes, scale, chunk_ids, chunk_size, start, rows, block):
+    device = scale.device
+    B, H, cap = _kv8_cache(codes, scale, "codes", block, device if not codes.is_cuda else codes.device)
+    out = torch.empty(B, H, rows, 128, dtype=torch.bfloat16, device=device)
+    with torch.cuda.device(device):
+        _lib.call("skv_kv8_read", device_address(codes), *_strides(codes, 3), scale.data_ptr(), *_strides(scale, 2),
+                  None if chunk_ids is None else chunk_ids.data_ptr(), chunk_size, start, out.data_ptr(), B, H, rows,
+                  cap, block, _stream())
+    return out
+
+
+def kv8_read(codes, scale, start, rows, *, block=64):
+    """Rows [start, start + rows) of one 8-bit cache [B, H, capacity, 128] as bf16 [B, H, rows, 128] (exact for
+    scales that kv8_write wrote, subnormal values apart). codes: a device tensor, or a pinned host one (read over
+    the host link, its scales on the device)."""
+    if rows < 1 or start < 0 or start + rows > codes.shape[2]:
+        raise ValueError(f"kv8_read: rows [{start}, {start + rows}) of {codes.shape[2]}")
+    return _kv8_read(codes, scale, None, 1, start, rows, block)
+
+
+def kv8_read_chunks(codes, scale, chunk_ids, chunk_size, *, block=64):
+    """The chunks of chunk_size rows named by chunk_ids [B, H, n] (int64) of one 8-bit cache as bf16
+    [B, H, n * chunk_size, 128], as kv8_read; rows outside the cache read as zeros."""
+    _dev(chunk_ids, "chunk_ids", torch.int64)
+    if chunk_ids.dim() != 3 or chunk_ids.shape[:2] != codes.shape[:2] or chunk_ids.numel() == 0 or \
+            not chunk_ids.is_contiguous() or chunk_ids.device != scale.device:
+        raise ValueError(f"kv8_read_chunks: chunk_ids {tuple(chunk_ids.shape)} must be contiguous [B, H, n] with its scales")
+    if chunk_size < 1 or chunk_ids.shape[2] * chunk_size > KV8_MAX_TOKENS:
+        raise ValueError(f"kv8_read_chunks: {chunk_ids.shape[2]} chunks of {chunk_size} rows")
+    return _kv8_read(codes, scale, chunk_ids, chunk_size, 0, chunk_ids.shape[2] * chunk_size, block)
+
+
+def kv8_attn(q, k8, v8, k_scale, v_scale, lengths, counts=None, *, block=64, scale=None, window=None, sinks=0):
+    """Attention of each sequence's last tokens over an 8-bit cache that holds them: q [B, Hq, T, 128] (bf16, any
+    strides) -> [B, T, Hq, 128]. Query t < counts[b] (T without counts) is at position lengths[b] - counts[b] + t
+    and sees the keys up to its own; with a window only the last `window` of those and the first `sinks` of the
+    sequence. lengths (tokens held, the new ones among them; clamped to [0, capacity]), counts: device int32 [B],
+    read when the kernels run. Queries that see nothing and those past counts[b] give zeros. What a query does
+    not see may hold anything, NaN too. scale: 1 / sqrt(128) by default."""
+    B, H, cap = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    _no_grad("kv8_attn", q)
+    q = _rows128(q, "q")
+    Hq, T = q.shape[1], q.shape[2]
+    if q.shape[0] != B or Hq % H or q.device != k8.device:
+        raise ValueError(f"kv8_attn: q {tuple(q.shape)} on {q.device} for caches of [{B}, {H}] on {k8.device}")
+    if window is not None and not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31 or (sinks and window is None):
+        raise ValueError(f"kv8_attn: window={window} sinks={sinks} (a window of at least 1; sinks need one)")
+    lp = _kv8_ints(lengths, "lengths", B, k8.device)
+    cp = None if counts is None else _kv8_ints(counts, "counts", B, k8.device)
+    out = torch.empty(B, T, Hq, 128, dtype=torch.bfloat16, device=q.device)
+    window = 0 if window is None else window
+    nbytes = _lib.lib().skv_kv8_attn_workspace_bytes(B, Hq, H, T, cap, window, sinks)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    with torch.cuda.device(k8.device):
+        _lib.call("skv_kv8_attn", q.data_ptr(), *_strides(q, 3), k8.data_ptr(), v8.data_ptr(), *_strides(k8, 3),
+                  k_scale.data_ptr(), v_scale.data_ptr(), *_strides(k_scale, 2), lp, cp, B, Hq, H, T, cap, block,
+                  1.0 / math.sqrt(128) if scale is None else float(scale), window, sinks, out.data_ptr(),
+                  None if ws is None else ws.data_ptr(), nbytes, _stream())
+    return out
 
 
 HBM_PROBE_TILE_BYTES = 65536
