@@ -1178,19 +1178,12 @@ def gather_copy_misses_to_slots(values, v_cache_buffer, miss_ids, cnts, miss_slo
 KV8_BLOCKS = (16, 32, 64, 128)
 KV8_MAX_TOKENS = 2 ** 30
 
+# These checks stand in front of calls of a few microseconds: the usual layouts pass on few attribute reads.
+
 
 def _no_grad(what: str, *tensors) -> None:
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
-
-
-def _rows128(t: torch.Tensor, name: str) -> torch.Tensor:
-    """t [B, heads, rows, 128] bf16 as it is where its rows can be read 16 bytes at a time, else a copy."""
-    _dev(t, name, torch.bfloat16)
-    if t.dim() != 4 or t.shape[3] != 128 or t.numel() == 0:
-        raise ValueError(f"{name} {tuple(t.shape)} must be [B, heads, rows, 128], none of them empty")
-    ok = t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(s % 8 for s in _strides(t, 3))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor, n: int) -> tuple:
@@ -1198,55 +1191,85 @@ def _strides(t: torch.Tensor, n: int) -> tuple:
     return tuple(st if sz > 1 else 0 for st, sz in zip(t.stride()[:n], t.shape))
 
 
-def _kv8_ints(t: torch.Tensor, name: str, B: int, device) -> int:
+def _rows128(t: torch.Tensor, name: str):
+    """t [B, heads, rows, 128] bf16, as it is where its rows can be read 16 bytes at a time, else a copy; and its
+    strides but the last."""
+    _dev(t, name, torch.bfloat16)
+    shape = t.shape
+    if len(shape) != 4 or shape[3] != 128 or 0 in shape:
+        raise ValueError(f"{name} {tuple(shape)} must be [B, heads, rows, 128], none of them empty")
+    sb, sh, st, se = t.stride()
+    if se == 1 and not (sb | sh | st) & 7 and not t.data_ptr() & 15:
+        return t, (sb, sh, st)
+    strides = _strides(t, 3)
+    if se != 1 or t.data_ptr() & 15 or any(s % 8 for s in strides):
+        t = t.clone(memory_format=torch.contiguous_format)
+        strides = _strides(t, 3)
+    return t, strides
+
+
+def _kv8_ints(t: torch.Tensor, name: str, B: int, index: int) -> int:
     _dev(t, name, torch.int32)
-    if t.shape != (B,) or not t.is_contiguous() or t.device != device:
-        raise ValueError(f"{name} must be {B} contiguous int32 on {device}, got {tuple(t.shape)} on {t.device}")
+    if t.dim() != 1 or t.shape[0] != B or not t.is_contiguous() or t.get_device() != index:
+        raise ValueError(f"{name} must be {B} contiguous int32 on the caches' device, got {tuple(t.shape)} on {t.device}")
     return t.data_ptr()
 
 
-def _kv8_cache(codes: torch.Tensor, scale: torch.Tensor, name: str, block: int, device=None):
-    """Checks one cache; returns (B, H, cap)."""
+def _kv8_cache(codes: torch.Tensor, scale: torch.Tensor, name: str, block: int):
+    """Checks one cache but for where its codes are; returns ((B, H, cap), strides of the codes, of the scales)."""
     if block not in KV8_BLOCKS:
         raise ValueError(f"block={block} must be one of {KV8_BLOCKS}")
     _dev(scale, f"{name} scale", torch.float32)
     if codes.dtype != torch.float8_e4m3fn:
         raise ValueError(f"{name} must be torch.float8_e4m3fn, got {codes.dtype}")
-    if codes.dim() != 4 or codes.shape[3] != 128 or codes.numel() == 0 or codes.stride(3) != 1 or \
-            codes.data_ptr() % 16 or any(s % 16 for s in _strides(codes, 3)):
-        raise ValueError(f"{name} {tuple(codes.shape)} must be [B, H, capacity, 128] with contiguous rows, 16-byte "
-                         "aligned (strides multiples of 16)")
-    B, H, cap, _ = codes.shape
+    shape = codes.shape
+    if len(shape) != 4 or shape[3] != 128 or 0 in shape or codes.stride(3) != 1 or codes.data_ptr() & 15:
+        raise ValueError(f"{name} {tuple(shape)} must be [B, H, capacity, 128] with contiguous rows, 16-byte aligned")
+    B, H, cap, _ = shape
     if cap > KV8_MAX_TOKENS:
         raise ValueError(f"{name} holds {cap} tokens (at most {KV8_MAX_TOKENS})")
-    if scale.dim() != 3 or scale.shape[:2] != (B, H) or scale.shape[2] < (cap + block - 1) // block or \
-            scale.stride(2) != 1:
-        raise ValueError(f"{name} scale {tuple(scale.shape)} must be [{B}, {H}, {(cap + block - 1) // block} or more] "
-                         "with contiguous rows")
-    if scale.device != (codes.device if device is None else device):
-        raise ValueError(f"{name} and its scale must be on one device")
-    return B, H, cap
+    if codes.is_contiguous():
+        strides = (H * cap * 128, cap * 128, 128)
+    else:
+        strides = _strides(codes, 3)
+        if any(s % 16 for s in strides):
+            raise ValueError(f"{name}: strides {strides} must be multiples of 16")
+    sshape, blocks = scale.shape, (cap + block - 1) // block
+    if len(sshape) != 3 or sshape[0] != B or sshape[1] != H or sshape[2] < blocks or scale.stride(2) != 1:
+        raise ValueError(f"{name} scale {tuple(sshape)} must be [{B}, {H}, {blocks} or more] with contiguous rows")
+    return (B, H, cap), strides, (H * sshape[2], sshape[2]) if scale.is_contiguous() else _strides(scale, 2)
 
 
 def _kv8_pair(k8, v8, k_scale, v_scale, block):
-    """Checks keys and values of one layout; returns (B, H, cap)."""
-    _dev(k8, "k8"), _dev(v8, "v8")
+    """Checks keys and values of one layout; returns ((B, H, cap), strides of codes, of scales, device index)."""
+    index = k8.get_device()
+    if index < 0 or v8.get_device() != index or k_scale.get_device() != index or v_scale.get_device() != index:
+        raise ValueError("k8, v8 and their scales must be on one device")
     geo = _kv8_cache(k8, k_scale, "k8", block)
-    _kv8_cache(v8, v_scale, "v8", block)
-    if k8.shape != v8.shape or _strides(k8, 3) != _strides(v8, 3) or \
-            _strides(k_scale, 2) != _strides(v_scale, 2) or k8.device != v8.device:
-        raise ValueError("k8 and v8 (and their scales) must share a layout and a device")
-    return geo
+    if geo != _kv8_cache(v8, v_scale, "v8", block):
+        raise ValueError("k8 and v8 (and their scales) must share a layout")
+    return *geo, index
 
 
 def _distinct(t: torch.Tensor) -> bool:
     """Whether no two elements of t can share memory."""
+    if t.is_contiguous():
+        return True
     extent = 1
     for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
         if stride < extent:
             return False
         extent += (size - 1) * stride
     return True
+
+
+def _call_on(index: int, name: str, *args) -> None:
+    """An entry point on a device's current stream, whichever device is current."""
+    if torch._C._cuda_getDevice() == index:
+        _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
@@ -1257,32 +1280,32 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
     A block's scale is the smallest power of two under which its new rows fit; where it holds older rows (before
     start[b]) it never falls, and they are encoded again where it grows. Infinities become NaN. Nothing else in
     the caches changes."""
-    B, H, cap = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    (B, H, cap), c_strides, s_strides, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
     _no_grad("kv8_write", k, v)
-    k, v = _rows128(k, "k"), _rows128(v, "v")
-    if k.shape != v.shape or k.shape[:2] != (B, H):
+    k, k_strides = _rows128(k, "k")
+    v, v_strides = _rows128(v, "v")
+    if k.shape != v.shape or k.shape[0] != B or k.shape[1] != H:
         raise ValueError(f"kv8_write: k {tuple(k.shape)} v {tuple(v.shape)} for caches of [{B}, {H}]")
-    if k.device != k8.device or v.device != k8.device:
+    if k.get_device() != index or v.get_device() != index:
         raise ValueError("kv8_write: rows and caches must be on one device")
-    if not all(_distinct(t) for t in (k8, v8, k_scale, v_scale)) or k8.data_ptr() == v8.data_ptr() or \
-            k_scale.data_ptr() == v_scale.data_ptr():
+    if not (_distinct(k8) and _distinct(v8) and _distinct(k_scale) and _distinct(v_scale)) or \
+            k8.data_ptr() == v8.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
         raise ValueError("kv8_write: the caches must not share memory with themselves or each other")
-    sp = _kv8_ints(start, "start", B, k8.device)
-    cp = None if counts is None else _kv8_ints(counts, "counts", B, k8.device)
-    with torch.cuda.device(k8.device):
-        _lib.call("skv_kv8_write", k.data_ptr(), *_strides(k, 3), v.data_ptr(), *_strides(v, 3), k8.data_ptr(),
-                  v8.data_ptr(), *_strides(k8, 3), k_scale.data_ptr(), v_scale.data_ptr(), *_strides(k_scale, 2), sp, cp,
-                  B, H, k.shape[2], cap, block, _stream())
+    sp = _kv8_ints(start, "start", B, index)
+    cp = None if counts is None else _kv8_ints(counts, "counts", B, index)
+    _call_on(index, "skv_kv8_write", k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, k8.data_ptr(), v8.data_ptr(),
+             *c_strides, k_scale.data_ptr(), v_scale.data_ptr(), *s_strides, sp, cp, B, H, k.shape[2], cap, block)
 
 
 def _kv8_read(codes, scale, chunk_ids, chunk_size, start, rows, block):
-    device = scale.device
-    B, H, cap = _kv8_cache(codes, scale, "codes", block, device if not codes.is_cuda else codes.device)
-    out = torch.empty(B, H, rows, 128, dtype=torch.bfloat16, device=device)
-    with torch.cuda.device(device):
-        _lib.call("skv_kv8_read", device_address(codes), *_strides(codes, 3), scale.data_ptr(), *_strides(scale, 2),
-                  None if chunk_ids is None else chunk_ids.data_ptr(), chunk_size, start, out.data_ptr(), B, H, rows,
-                  cap, block, _stream())
+    (B, H, cap), c_strides, s_strides = _kv8_cache(codes, scale, "codes", block)
+    index = scale.get_device()
+    if codes.is_cuda and codes.get_device() != index:
+        raise ValueError("the codes and their scales must be on one device")
+    out = torch.empty(B, H, rows, 128, dtype=torch.bfloat16, device=scale.device)
+    _call_on(index, "skv_kv8_read", device_address(codes), *c_strides, scale.data_ptr(), *s_strides,
+             None if chunk_ids is None else chunk_ids.data_ptr(), chunk_size, start, out.data_ptr(), B, H, rows, cap,
+             block)
     return out
 
 
@@ -1290,8 +1313,8 @@ def kv8_read(codes, scale, start, rows, *, block=64):
     """Rows [start, start + rows) of one 8-bit cache [B, H, capacity, 128] as bf16 [B, H, rows, 128] (exact for
     scales that kv8_write wrote, subnormal values apart). codes: a device tensor, or a pinned host one (read over
     the host link, its scales on the device)."""
-    if rows < 1 or start < 0 or start + rows > codes.shape[2]:
-        raise ValueError(f"kv8_read: rows [{start}, {start + rows}) of {codes.shape[2]}")
+    if rows < 1 or start < 0 or codes.dim() != 4 or start + rows > codes.shape[2]:
+        raise ValueError(f"kv8_read: rows [{start}, {start + rows}) of codes {tuple(codes.shape)}")
     return _kv8_read(codes, scale, None, 1, start, rows, block)
 
 
@@ -1299,12 +1322,18 @@ def kv8_read_chunks(codes, scale, chunk_ids, chunk_size, *, block=64):
     """The chunks of chunk_size rows named by chunk_ids [B, H, n] (int64) of one 8-bit cache as bf16
     [B, H, n * chunk_size, 128], as kv8_read; rows outside the cache read as zeros."""
     _dev(chunk_ids, "chunk_ids", torch.int64)
-    if chunk_ids.dim() != 3 or chunk_ids.shape[:2] != codes.shape[:2] or chunk_ids.numel() == 0 or \
-            not chunk_ids.is_contiguous() or chunk_ids.device != scale.device:
-        raise ValueError(f"kv8_read_chunks: chunk_ids {tuple(chunk_ids.shape)} must be contiguous [B, H, n] with its scales")
-    if chunk_size < 1 or chunk_ids.shape[2] * chunk_size > KV8_MAX_TOKENS:
-        raise ValueError(f"kv8_read_chunks: {chunk_ids.shape[2]} chunks of {chunk_size} rows")
-    return _kv8_read(codes, scale, chunk_ids, chunk_size, 0, chunk_ids.shape[2] * chunk_size, block)
+    shape = chunk_ids.shape
+    if len(shape) != 3 or shape[:2] != codes.shape[:2] or 0 in shape or not chunk_ids.is_contiguous() or \
+            chunk_ids.get_device() != scale.get_device():
+        raise ValueError(f"kv8_read_chunks: chunk_ids {tuple(shape)} must be contiguous [B, H, n], with the scales")
+    if chunk_size < 1 or shape[2] * chunk_size > KV8_MAX_TOKENS:
+        raise ValueError(f"kv8_read_chunks: {shape[2]} chunks of {chunk_size} rows")
+    return _kv8_read(codes, scale, chunk_ids, chunk_size, 0, shape[2] * chunk_size, block)
+
+
+@functools.lru_cache(maxsize=256)
+def _kv8_attn_workspace_bytes(B, Hq, H, T, cap, window, sinks) -> int:
+    return int(_lib.lib().skv_kv8_attn_workspace_bytes(B, Hq, H, T, cap, window, sinks))
 
 
 def kv8_attn(q, k8, v8, k_scale, v_scale, lengths, counts=None, *, block=64, scale=None, window=None, sinks=0):
@@ -1314,25 +1343,24 @@ def kv8_attn(q, k8, v8, k_scale, v_scale, lengths, counts=None, *, block=64, sca
     sequence. lengths (tokens held, the new ones among them; clamped to [0, capacity]), counts: device int32 [B],
     read when the kernels run. Queries that see nothing and those past counts[b] give zeros. What a query does
     not see may hold anything, NaN too. scale: 1 / sqrt(128) by default."""
-    B, H, cap = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    (B, H, cap), c_strides, s_strides, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
     _no_grad("kv8_attn", q)
-    q = _rows128(q, "q")
-    Hq, T = q.shape[1], q.shape[2]
-    if q.shape[0] != B or Hq % H or q.device != k8.device:
+    q, q_strides = _rows128(q, "q")
+    Bq, Hq, T, _ = q.shape
+    if Bq != B or Hq % H or q.get_device() != index:
         raise ValueError(f"kv8_attn: q {tuple(q.shape)} on {q.device} for caches of [{B}, {H}] on {k8.device}")
     if window is not None and not 1 <= window < 2 ** 31 or not 0 <= sinks < 2 ** 31 or (sinks and window is None):
         raise ValueError(f"kv8_attn: window={window} sinks={sinks} (a window of at least 1; sinks need one)")
-    lp = _kv8_ints(lengths, "lengths", B, k8.device)
-    cp = None if counts is None else _kv8_ints(counts, "counts", B, k8.device)
-    out = torch.empty(B, T, Hq, 128, dtype=torch.bfloat16, device=q.device)
+    lp = _kv8_ints(lengths, "lengths", B, index)
+    cp = None if counts is None else _kv8_ints(counts, "counts", B, index)
     window = 0 if window is None else window
-    nbytes = _lib.lib().skv_kv8_attn_workspace_bytes(B, Hq, H, T, cap, window, sinks)
+    out = torch.empty(B, T, Hq, 128, dtype=torch.bfloat16, device=q.device)
+    nbytes = _kv8_attn_workspace_bytes(B, Hq, H, T, cap, window, sinks)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    with torch.cuda.device(k8.device):
-        _lib.call("skv_kv8_attn", q.data_ptr(), *_strides(q, 3), k8.data_ptr(), v8.data_ptr(), *_strides(k8, 3),
-                  k_scale.data_ptr(), v_scale.data_ptr(), *_strides(k_scale, 2), lp, cp, B, Hq, H, T, cap, block,
-                  1.0 / math.sqrt(128) if scale is None else float(scale), window, sinks, out.data_ptr(),
-                  None if ws is None else ws.data_ptr(), nbytes, _stream())
+    _call_on(index, "skv_kv8_attn", q.data_ptr(), *q_strides, k8.data_ptr(), v8.data_ptr(), *c_strides,
+             k_scale.data_ptr(), v_scale.data_ptr(), *s_strides, lp, cp, B, Hq, H, T, cap, block,
+             1.0 / math.sqrt(128) if scale is None else float(scale), window, sinks, out.data_ptr(),
+             None if ws is None else ws.data_ptr(), nbytes)
     return out
 
 
