@@ -10,6 +10,8 @@
 // enters the product with the values as two bf16 parts (16 significant bits, an error of 2^-16 where the output's
 // one rounding is 2^-9).
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "skv_common.h"
 
@@ -19,6 +21,9 @@ using skv::u32x4;
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -40,7 +45,8 @@ struct Args {
   float* ws_o;
   float* ws_ml;
   int B, H, G, T, cap, block_shift, window, sinks;
-  float scale_log2e;
+  float scale_log2e;  // of the scale's magnitude
+  bool negative;      // whether the scale is: the queries' sign is turned instead
   int target;   // one token: workgroups to aim for
   int splits;   // many: shares of a row tile's keys
   int rtiles;   // many: row tiles of a (sequence, kv head)
@@ -70,6 +76,17 @@ __device__ __forceinline__ bool sees(int p, int j, int window, int sinks) {
   return j <= p && (j > p - window || j < sinks);
 }
 
+// A scale at a wave-uniform place, through the scalar unit (nothing writes the scales while these kernels run).
+__device__ __forceinline__ float scale_at(const float* scales, int block) {
+  return *reinterpret_cast<const __attribute__((address_space(4))) float*>(reinterpret_cast<uintptr_t>(scales + block));
+}
+
+// A key block's factor of its scores, in units of log2: positive, so that a hidden key's -inf stays one.
+__device__ __forceinline__ float key_factor(float scale, float scale_log2e) {
+  const float f = scale * scale_log2e;
+  return f < 1.17549435e-38f ? 1.17549435e-38f : f;  // (NaN stays NaN)
+}
+
 __device__ __forceinline__ bf16x8 bf16_of(uint32_t a, uint32_t b) {
   u32x4 o;
   o[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.f, false));
@@ -89,6 +106,19 @@ __device__ __forceinline__ void transpose_bf16(const uint32_t (&w)[8], u32x4 (&o
     o[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true));
     o[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false));
     o[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true));
+  }
+}
+
+// The same as f16 of code * factor (a power of two).
+__device__ __forceinline__ void transpose_f16(const uint32_t (&w)[8], float factor, u32x4 (&o)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t lo = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05010400u);
+    const uint32_t hi = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07030602u);
+    o[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, factor, false));
+    o[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, factor, true));
+    o[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, factor, false));
+    o[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, factor, true));
   }
 }
 
@@ -185,7 +215,8 @@ __global__ void __launch_bounds__(256) token_kernel(Args a) {
     const uint16_t* q = a.q + b * a.q_sb + (h * G + min(li, G - 1)) * a.q_sh + 16 * grp;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      qf[s] = __builtin_bit_cast(bf16x8, skv::load16_or_zero(q + 64 * (s >> 1) + 8 * (s & 1), li < G));
+      qf[s] = __builtin_bit_cast(bf16x8, skv::load16_or_zero(q + 64 * (s >> 1) + 8 * (s & 1), li < G) ^
+                                             (a.negative ? 0x80008000u : 0u));
   }
   const uint8_t* kh = a.k8 + b * a.c_sb + h * a.c_sh + 16 * grp;
   const uint8_t* vh = a.v8 + b * a.c_sb + h * a.c_sh + 8 * li;
@@ -230,7 +261,7 @@ __global__ void __launch_bounds__(256) token_kernel(Args a) {
       for (int st = 0; st < 4; ++st)
         s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
             bf16_of(kr[u][st >> 1][2 * (st & 1)], kr[u][st >> 1][2 * (st & 1) + 1]), qf[st], s[u], 0, 0, 0);
-      const float f = kc[u] * a.scale_log2e;
+      const float f = key_factor(kc[u], a.scale_log2e);
 #pragma unroll
       for (int r = 0; r < 4; ++r) s[u][r] *= f;
     }
@@ -393,11 +424,20 @@ __device__ __forceinline__ u32x4 load4(const uint8_t* p) { return *reinterpret_c
 // 0x80 in each byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
+// Powers of two by which the value blocks of a workgroup may differ for f16 to hold their values exactly, and the
+// one that the largest block's codes are raised by: 448 * 2^7 is just below f16's largest, 2^-9 * 2^(7 - 12) its
+// smallest normal value.
+constexpr int kSpread = 12;
+constexpr int kRaise = 7;
+// A probability is at most 2^(kRaise + kSlack), below f16's largest: kSlack is how far a score may pass the reference.
+constexpr float kSlack = 8.f;
+
 __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   __shared__ u32x4 kt[2][kTile * 16], vt[2][kTile * 16];
   // Values that are NaN, by (buffer, wave that carries them): whether there are any, and each dim's keys as bits.
   __shared__ int odd_lds[2][2];
   __shared__ uint32_t odd_keys[2][2][kD];
+  __shared__ int vexp[3];  // largest and smallest exponent of the value blocks' scales, whether one is no power of two
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int li = lane & 31, half = lane >> 5;
@@ -432,6 +472,9 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     const uint16_t* q = a.q + b * a.q_sb + (h * G + g) * a.q_sh + t * a.q_st + 8 * half;
 #pragma unroll
     for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
+    if (a.negative)
+#pragma unroll
+      for (int s = 0; s < 8; ++s) qf[s] ^= 0x80008000u;
   }
   const uint8_t* kh = a.k8 + b * a.c_sb + h * a.c_sh;
   const uint8_t* vh = a.v8 + b * a.c_sb + h * a.c_sh;
@@ -443,24 +486,36 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   const int x = threadIdx.x & 127;
   const int krow = x >> 1, kpart = x & 1;
   const int vgk = x >> 5, vhalf = (x >> 4) & 1, vc = x & 15;
+  // Row offsets of the thread in a tile; rows behind the sequence's end are out of the buffer's bounds and come as
+  // zeros, whatever lies there.
+  const int stride = static_cast<int>(a.c_ss);
+  const int mine = wave < 2 ? krow * stride + 64 * kpart : (16 * vgk + 4 * vhalf) * stride + 8 * vc;
   u32x4 held[4];
+  float kf[4], kn[4];  // this tile's and the next one's key factors
   auto fetch = [&](int tile) __attribute__((always_inline)) {
-    const int j0 = tile * kTile;
+    const int64_t j0 = static_cast<int64_t>(tile) * kTile;
+    const int bytes = min(len - tile * kTile - 1, kTile - 1) * stride + kD;
+    constexpr int kDw3 = 0x00020000;  // buffer resource word 3 (gfx9)
     if (wave < 2) {
-      const uint8_t* src = kh + static_cast<int64_t>(min(j0 + krow, len - 1)) * a.c_ss + 64 * kpart;
+      const __amdgpu_buffer_rsrc_t src =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kh + j0 * a.c_ss), 0, bytes, kDw3);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) held[c] = load4(src + 16 * c);
+      for (int c = 0; c < 4; ++c) held[c] = __builtin_amdgcn_raw_buffer_load_b128(src, mine, 16 * c, 0);
     } else {
+      const __amdgpu_buffer_rsrc_t src =
+          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vh + j0 * a.c_ss), 0, bytes, kDw3);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const int j = j0 + 16 * vgk + 4 * vhalf + (e & 3) + 8 * (e >> 2);
-        const u32x2 w = *reinterpret_cast<const u32x2*>(vh + static_cast<int64_t>(min(j, len - 1)) * a.c_ss + 8 * vc);
-        held[e >> 1][2 * (e & 1)] = j < len ? w[0] : 0u;  // (what lies behind the sequence may be anything)
-        held[e >> 1][2 * (e & 1) + 1] = j < len ? w[1] : 0u;
+        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(src, mine, ((e & 3) + 8 * (e >> 2)) * stride, 0);
+        held[e >> 1][2 * (e & 1)] = w[0];
+        held[e >> 1][2 * (e & 1) + 1] = w[1];
       }
     }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      kn[q] = key_factor(scale_at(ksh, min(tile * kTile + 16 * q, len - 1) >> a.block_shift), a.scale_log2e);
   };
-  auto place = [&](int buf) __attribute__((always_inline)) {
+  auto place = [&](auto f16, float factor, int buf) __attribute__((always_inline)) {
     if (wave < 2) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -468,13 +523,16 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
         kt[buf][k_at(krow, 8 * kpart + 2 * c + 1)] = __builtin_bit_cast(u32x4, bf16_of(held[c][2], held[c][3]));
       }
     } else {
-      uint32_t odd = 0;
+      bool any = false;
+      if constexpr (!decltype(f16)::value) {
+        uint32_t odd = 0;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) odd |= nan_bytes(held[c][e]);
-      const bool any = __any(odd != 0);
-      if (lane == 0) odd_lds[buf][wave - 2] = any;
+          for (int e = 0; e < 4; ++e) odd |= nan_bytes(held[c][e]);
+        any = __any(odd != 0);
+        if (lane == 0) odd_lds[buf][wave - 2] = any;
+      }
       if (any) {  // wave-uniform: their keys are noted, and they enter the products as zeros
         uint32_t* keys = odd_keys[buf][wave - 2];
         keys[lane] = 0u;
@@ -499,7 +557,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = held[e >> 1][2 * (e & 1) + hf];
         u32x4 o[4];
-        transpose_bf16(w, o);
+        if constexpr (decltype(f16)::value) transpose_f16(w, factor, o);
+        else transpose_bf16(w, o);
 #pragma unroll
         for (int e = 0; e < 4; ++e) vt[buf][v_at(vgk, vhalf, 8 * vc + 4 * hf + e)] = o[e];
       }
@@ -507,14 +566,11 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   };
 
   f32x16 o[4];
-#pragma unroll
-  for (int d = 0; d < 4; ++d)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-  float m = -INFINITY, l = 0.f;
+  float m, l;
   uint64_t odd = 0;  // this lane's output dims that a value seen by its row makes NaN, bit 16 d + r
 
-  auto compute = [&](int tile, int buf) __attribute__((always_inline)) {
+  auto compute = [&](auto f16, int tile, int buf) __attribute__((always_inline)) {
+    constexpr bool kF16 = decltype(f16)::value;
     const int k0 = tile * kTile;
     // wave-uniform: nothing of the tile is seen
     if (k0 > wmax || (k0 + kTile <= wmin - a.window + 1 && k0 >= a.sinks)) return;
@@ -531,15 +587,6 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
             __builtin_bit_cast(bf16x8, kt[buf][k_at(32 * u + li, 2 * c + half)]), __builtin_bit_cast(bf16x8, qf[c]),
             s[u], 0, 0, 0);
     // Registers 8 i to 8 i + 7 of s[u] hold 8 of the keys 32 u + 16 i to 32 u + 16 i + 15, which share a block.
-    float vsc[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int blk = min(k0 + 16 * q, len - 1) >> a.block_shift;
-      const float f = ksh[blk] * a.scale_log2e;
-      vsc[q] = vsh[blk];
-#pragma unroll
-      for (int r = 0; r < 8; ++r) s[q >> 1][8 * (q & 1) + r] *= f;
-    }
     const bool all = whole && k0 + kTile - 1 <= wmin && (k0 > wmax - a.window || k0 + kTile <= a.sinks);
     if (!all) {  // wave-uniform
 #pragma unroll
@@ -548,16 +595,20 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
         for (int r = 0; r < 16; ++r)
           if (!sees(p, k0 + 32 * u + 8 * (r / 4) + 4 * half + (r % 4), a.window, a.sinks)) s[u][r] = -INFINITY;
     }
-    float mx = s[0][0];
+    float mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+    for (int q = 0; q < 4; ++q) {
+      float y = s[q >> 1][8 * (q & 1)];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
+      for (int r = 1; r < 8; ++r) y = fmaxf(y, s[q >> 1][8 * (q & 1) + r]);
+      mx = fmaxf(mx, y * kf[q]);
+    }
     {
       const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
       mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
     }
-    if (__any(mx > m)) {  // wave-uniform
+    // The reference moves only when a score passes it by 2^kSlack: the ratio of the sums does not depend on it.
+    if (__any(mx > m + kSlack)) {  // wave-uniform
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
@@ -567,15 +618,15 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= f;
     }
-    const float ref = m == -INFINITY ? 0.f : m;
+    const float ref = (m == -INFINITY ? 0.f : m) - static_cast<float>(kRaise);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[u][r] = __builtin_amdgcn_exp2f(s[u][r] - ref);
+        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], kf[2 * u + (r >> 3)], -ref));
         l += s[u][r];
       }
-    if (odd_lds[buf][0] | odd_lds[buf][1]) {  // the same for all waves
+    if (!kF16 && (odd_lds[buf][0] | odd_lds[buf][1])) {  // the same for all waves
       // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
       // would: a hidden key's zero times NaN).
       for (int hw = 0; hw < 2; ++hw) {
@@ -588,37 +639,108 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     }
 #pragma unroll
     for (int gk = 0; gk < 4; ++gk) {
-      u32x4 part[2];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t first, second;
-        two_parts(s[gk >> 1][8 * (gk & 1) + 2 * e] * vsc[gk], s[gk >> 1][8 * (gk & 1) + 2 * e + 1] * vsc[gk], first,
-                  second);
-        part[0][e] = first;
-        part[1][e] = second;
-      }
       u32x4 vf[4];
 #pragma unroll
       for (int d = 0; d < 4; ++d) vf[d] = vt[buf][v_at(gk, half, 32 * d + li)];
+      if constexpr (kF16) {
+        u32x4 part;
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+        for (int e = 0; e < 4; ++e)
+          part[e] = __builtin_bit_cast(
+              uint32_t, __builtin_convertvector(f32x2{s[gk >> 1][8 * (gk & 1) + 2 * e],
+                                                      s[gk >> 1][8 * (gk & 1) + 2 * e + 1]}, f16x2));
 #pragma unroll
         for (int d = 0; d < 4; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[d]),
-                                                         __builtin_bit_cast(bf16x8, part[y]), o[d], 0, 0, 0);
+          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf[d]),
+                                                        __builtin_bit_cast(f16x8, part), o[d], 0, 0, 0);
+      } else {
+        __builtin_amdgcn_sched_barrier(0);  // (one group's operands at a time: registers)
+        const float vsc = scale_at(vsh, min(k0 + 16 * gk, len - 1) >> a.block_shift);
+        u32x4 part[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t first, second;
+          two_parts(s[gk >> 1][8 * (gk & 1) + 2 * e] * vsc, s[gk >> 1][8 * (gk & 1) + 2 * e + 1] * vsc, first, second);
+          part[0][e] = first;
+          part[1][e] = second;
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
+#pragma unroll
+          for (int d = 0; d < 4; ++d)
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[d]),
+                                                           __builtin_bit_cast(bf16x8, part[y]), o[d], 0, 0, 0);
+      }
     }
   };
 
-  if (i0 < i1) {  // workgroup-uniform
+  // Whether f16 holds this workgroup's values: blocks of scales that are powers of two and near one another (those
+  // at the smallest, 2^-126, are zeros beside any other).
+  if (threadIdx.x < 3) vexp[threadIdx.x] = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? 255 : 0;
+  __syncthreads();
+  for (int i = 4 * i0 + threadIdx.x; i < 4 * i1; i += 256) {
+    const uint32_t v = __float_as_uint(vsh[min(seen.at(i >> 2) * kTile + 16 * (i & 3), len - 1) >> a.block_shift]);
+    const int e = static_cast<int>(v >> 23);
+    if (v > 0x00800000u) {
+      atomicMax(&vexp[0], e);
+      atomicMin(&vexp[1], e);
+      if (v & 0x807fffffu) vexp[2] = 1;
+    }
+  }
+  __syncthreads();
+  const int vtop = vexp[0];
+  const bool fits = !vexp[2] && vtop < 255 && vtop - vexp[1] <= kSpread;  // the same for all
+  auto walk = [&](auto f16) __attribute__((always_inline)) {
+    // The factor of the wave's value blocks: a group of 16 keys a half wave.
+    auto factor = [&](int tile) __attribute__((always_inline)) {
+      const uint32_t v = __float_as_uint(vsh[min(tile * kTile + 16 * vgk, len - 1) >> a.block_shift]);
+      return __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(v >> 23) - vtop + 127 + kRaise, 1)) << 23);
+    };
+    float next = 1.f;
     fetch(seen.at(i0));
-    place(0);
+    if constexpr (decltype(f16)::value) next = factor(seen.at(i0));
+    place(f16, next, 0);
     for (int i = i0; i < i1; ++i) {
       const int buf = (i - i0) & 1;
       // Tile i is in buf, and every wave is past tile i - 1 in the other one.
       __syncthreads();
-      if (i + 1 < i1) fetch(seen.at(i + 1));
-      compute(seen.at(i), buf);
-      if (i + 1 < i1) place(buf ^ 1);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) kf[q] = kn[q];
+      if (i + 1 < i1) {
+        fetch(seen.at(i + 1));
+        if constexpr (decltype(f16)::value) next = factor(seen.at(i + 1));
+      }
+      compute(f16, seen.at(i), buf);
+      if (i + 1 < i1) place(f16, next, buf ^ 1);
+    }
+  };
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  };
+  clear();
+  float back = 1.f;  // what the values' sums are multiplied with in the end
+  if (i0 < i1) {     // workgroup-uniform
+    bool exact = fits;
+    if (fits) {
+      walk(std::true_type{});
+      back = __builtin_ldexpf(1.f, vtop - 127 - kRaise);
+      // NaN anywhere: a value may have reached rows that do not see it.
+      bool odd = false;
+#pragma unroll
+      for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) odd |= o[d][r] != o[d][r];
+      exact = !__syncthreads_or(odd);
+    }
+    if (!exact) {
+      clear();
+      back = 1.f;
+      walk(std::false_type{});
     }
   }
 
@@ -630,7 +752,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = (odd >> (16 * d + r)) & 1 ? __builtin_nanf("") : o[d][r];
+    for (int r = 0; r < 16; ++r) o[d][r] = (odd >> (16 * d + r)) & 1 ? __builtin_nanf("") : o[d][r] * back;
   if (a.splits == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // (nothing seen: zeros)
     uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H * G + h * G + g) * kD + 4 * half;
@@ -738,6 +860,11 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
     skv_set_error("%s: rows of q, of the caches and of out must be 16-byte aligned", what);
     return SKV_EINVAL;
   }
+  if (cap == 1) c_stride_s = kD;  // (of no meaning)
+  if (c_stride_s < kD || c_stride_s > (1 << 24)) {
+    skv_set_error("%s: tokens %lld bytes apart (128 to 2^24)", what, (long long)c_stride_s);
+    return SKV_EUNSUPPORTED;
+  }
   const Plan p = plan_of(batch_size, kv_heads, q_heads / kv_heads, rows, cap, window, sinks);
   const int64_t need = p.parts * (kD + 2) * 4;
   if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 16))) {
@@ -755,7 +882,7 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
   Args a{q, q_stride_b, q_stride_h, q_stride_t, k8, v8, c_stride_b, c_stride_h, c_stride_s, k_scale, v_scale,
          s_stride_b, s_stride_h, lengths, counts, out, ws_o, ws_o ? ws_o + p.parts * kD : nullptr, batch_size,
          kv_heads, q_heads / kv_heads, rows, cap, shift, window ? std::min(window, kNoWindow) : kNoWindow, sinks,
-         scale * 1.44269504088896340736f, kTarget, p.splits, p.rtiles};
+         std::fabs(scale) * 1.44269504088896340736f, scale < 0.f, kTarget, p.splits, p.rtiles};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(p.grid)), t(256);
   if (p.token) {
