@@ -62,6 +62,9 @@ __device__ __forceinline__ int count_of(const Args& a, int b) {
 struct Groups {
   int first, skip, total;
   __device__ __forceinline__ int at(int i) const { return i < first ? i : i + skip; }
+  __device__ __forceinline__ int index(int group) const {  // of the first group at or behind `group`
+    return group < first ? group : max(first, group - skip);
+  }
 };
 __device__ __forceinline__ Groups groups_seen(int pmin, int pmax, int window, int sinks, int shift) {
   if (pmax < 0) return {0, 0, 0};
@@ -109,17 +112,12 @@ __device__ __forceinline__ void transpose_bf16(const uint32_t (&w)[8], u32x4 (&o
   }
 }
 
-// The same as f16 of code * factor (a power of two).
-__device__ __forceinline__ void transpose_f16(const uint32_t (&w)[8], float factor, u32x4 (&o)[4]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t lo = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x05010400u);
-    const uint32_t hi = __builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x07030602u);
-    o[0][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, factor, false));
-    o[1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, factor, true));
-    o[2][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, factor, false));
-    o[3][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, factor, true));
-  }
+// Dims 2 y and 2 y + 1 of the same, tokens 2 i and 2 i + 1, as f16 of code * factor (a power of two).
+__device__ __forceinline__ void f16_pair(uint32_t even, uint32_t odd, float factor, int y, int i, u32x4& o0,
+                                         u32x4& o1) {
+  const uint32_t w = __builtin_amdgcn_perm(odd, even, y ? 0x07030602u : 0x05010400u);
+  o0[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, factor, false));
+  o1[i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, factor, true));
 }
 
 // Two fp32 as two bf16 parts each: part[0] cut off, part[1] what that leaves, rounded.
@@ -421,6 +419,24 @@ __device__ __forceinline__ int v_at(int gk, int half, int d) { return gk * 256 +
 
 __device__ __forceinline__ u32x4 load4(const uint8_t* p) { return *reinterpret_cast<const u32x4*>(p); }
 
+// The largest of eight, four instructions (fmaxf would first quiet each operand that comes from a matrix instruction).
+// Not right behind the one that makes them: the compiler does not see what this waits for.
+__device__ __forceinline__ float max8(const f32x16& v, int r) {
+  float o;
+  asm("v_max3_f32 %0, %1, %2, %3\n\tv_max3_f32 %0, %0, %4, %5\n\tv_max3_f32 %0, %0, %6, %7\n\tv_max_f32 %0, %0, %8"
+      : "=&v"(o)
+      : "v"(v[r]), "v"(v[r + 1]), "v"(v[r + 2]), "v"(v[r + 3]), "v"(v[r + 4]), "v"(v[r + 5]), "v"(v[r + 6]),
+        "v"(v[r + 7]));
+  return o;
+}
+
+// A barrier for what goes through LDS: loads from memory stay on their way.
+__device__ __forceinline__ void barrier_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // 0x80 in each byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
@@ -435,12 +451,11 @@ constexpr float kSlack = 8.f;
 __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   __shared__ u32x4 kt[2][kTile * 16], vt[2][kTile * 16];
   // Values that are NaN, by (buffer, wave that carries them): whether there are any, and each dim's keys as bits.
-  __shared__ int odd_lds[2][2];
-  __shared__ uint32_t odd_keys[2][2][kD];
+  __shared__ int odd_lds[2][4];
+  __shared__ uint32_t odd_keys[2][4][kD];
   __shared__ int vexp[3];  // largest and smallest exponent of the value blocks' scales, whether one is no power of two
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int li = lane & 31, half = lane >> 5;
   int i = blockIdx.x;
   const int BH = a.B * a.H;
   const int bh = i % BH;
@@ -459,17 +474,24 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   const int each = (seen.total + a.splits - 1) / a.splits;
   const int i0 = min(split * each, seen.total), i1 = min(i0 + each, seen.total);
 
-  const int row = r0 + wave * kRowsWave + li;
-  const int t = min(row, R - 1) / G, g = min(row, R - 1) - t * G;
-  const int p = row < R && t < n ? p0 + t : -1;
-  // the wave's positions (wave-uniform): rows past the last or of padding do not widen them
-  const int wr = r0 + wave * kRowsWave;
-  const int wmin = p0 + wr / G, wmax = wr / G < n ? p0 + min(n - 1, (wr + kRowsWave - 1) / G) : -1;
-  const bool whole = wr + kRowsWave <= R && (wr + kRowsWave - 1) / G < n;  // every row of the wave is a query
-
+  // Row li of the wave: query t, head g of the kv head's. Those past the last row, and of padding, ride along with the
+  // last query, and give nothing in the end.
+  struct Row {
+    int row, t, g;
+    bool query;
+  };
+  auto row_of = [&](int li) __attribute__((always_inline)) {
+    Row x;
+    x.row = r0 + wave * kRowsWave + li;
+    x.t = min(x.row, R - 1) / G;
+    x.g = min(x.row, R - 1) - x.t * G;
+    x.query = x.row < R && x.t < n;
+    return x;
+  };
   u32x4 qf[8];
   {
-    const uint16_t* q = a.q + b * a.q_sb + (h * G + g) * a.q_sh + t * a.q_st + 8 * half;
+    const Row x = row_of(threadIdx.x & 31);
+    const uint16_t* q = a.q + b * a.q_sb + (h * G + x.g) * a.q_sh + x.t * a.q_st + 8 * (lane >> 5);
 #pragma unroll
     for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
     if (a.negative)
@@ -481,120 +503,107 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   const float* ksh = a.ks + b * a.s_sb + h * a.s_sh;
   const float* vsh = a.vs + b * a.s_sb + h * a.s_sh;
 
-  // Waves 0 and 1 carry the keys (a thread 64 bytes of a row), waves 2 and 3 the values (a thread 8 dims of the 8
-  // tokens of a half group, the keys' order in the scores' registers).
-  const int x = threadIdx.x & 127;
-  const int krow = x >> 1, kpart = x & 1;
-  const int vgk = x >> 5, vhalf = (x >> 4) & 1, vc = x & 15;
-  // Row offsets of the thread in a tile; rows behind the sequence's end are out of the buffer's bounds and come as
-  // zeros, whatever lies there.
+  // A thread carries 32 bytes of a key row, and four dims of the values of 8 tokens: half of a group of 16, a wave's,
+  // in the order of the keys in the scores' registers. Rows behind the sequence's end are out of the buffer's bounds
+  // and come as zeros, whatever lies there.
   const int stride = static_cast<int>(a.c_ss);
-  const int mine = wave < 2 ? krow * stride + 64 * kpart : (16 * vgk + 4 * vhalf) * stride + 8 * vc;
-  u32x4 held[4];
-  float kf[4], kn[4];  // this tile's and the next one's key factors
-  auto fetch = [&](int tile) __attribute__((always_inline)) {
-    const int64_t j0 = static_cast<int64_t>(tile) * kTile;
-    const int bytes = min(len - tile * kTile - 1, kTile - 1) * stride + kD;
-    constexpr int kDw3 = 0x00020000;  // buffer resource word 3 (gfx9)
-    if (wave < 2) {
-      const __amdgpu_buffer_rsrc_t src =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(kh + j0 * a.c_ss), 0, bytes, kDw3);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) held[c] = __builtin_amdgcn_raw_buffer_load_b128(src, mine, 16 * c, 0);
-    } else {
-      const __amdgpu_buffer_rsrc_t src =
-          __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(vh + j0 * a.c_ss), 0, bytes, kDw3);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const u32x2 w = __builtin_amdgcn_raw_buffer_load_b64(src, mine, ((e & 3) + 8 * (e >> 2)) * stride, 0);
-        held[e >> 1][2 * (e & 1)] = w[0];
-        held[e >> 1][2 * (e & 1) + 1] = w[1];
-      }
-    }
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      kn[q] = key_factor(scale_at(ksh, min(tile * kTile + 16 * q, len - 1) >> a.block_shift), a.scale_log2e);
+  struct Lane {
+    int li, half, krow, kpart, kmine, vmine;
   };
-  auto place = [&](auto f16, float factor, int buf) __attribute__((always_inline)) {
-    if (wave < 2) {
+  // (made anew where a walk begins, from a thread id that the compiler takes for another one: what hangs on it would
+  // else be held in registers from walk to walk)
+  auto own_lane = [&]() __attribute__((always_inline)) {
+    int tid = threadIdx.x;
+    asm volatile("" : "+v"(tid));
+    Lane x;
+    x.li = tid & 31;
+    x.half = (tid >> 5) & 1;
+    x.krow = tid >> 2;
+    x.kpart = tid & 3;
+    x.kmine = x.krow * stride + 32 * x.kpart;
+    x.vmine = (16 * wave + 4 * x.half) * stride + 4 * x.li;
+    return x;
+  };
+  constexpr int kDw3 = 0x00020000;  // buffer resource word 3 (gfx9)
+  auto tile_rows = [&](const uint8_t* base, int tile) __attribute__((always_inline)) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + static_cast<int64_t>(tile) * kTile * a.c_ss), 0,
+                                             min(len - tile * kTile - 1, kTile - 1) * stride + kD, kDw3);
+  };
+  u32x4 kheld[2];
+  uint32_t vheld[8];
+  auto fetch_keys = [&](const Lane& x, int tile) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t src = tile_rows(kh, tile);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        kt[buf][k_at(krow, 8 * kpart + 2 * c)] = __builtin_bit_cast(u32x4, bf16_of(held[c][0], held[c][1]));
-        kt[buf][k_at(krow, 8 * kpart + 2 * c + 1)] = __builtin_bit_cast(u32x4, bf16_of(held[c][2], held[c][3]));
-      }
-    } else {
-      bool any = false;
-      if constexpr (!decltype(f16)::value) {
-        uint32_t odd = 0;
+    for (int c = 0; c < 2; ++c) kheld[c] = __builtin_amdgcn_raw_buffer_load_b128(src, x.kmine, 16 * c, 0);
+  };
+  auto fetch_values = [&](const Lane& x, int tile) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t src = tile_rows(vh, tile);
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+    for (int e = 0; e < 8; ++e)
+      vheld[e] = __builtin_amdgcn_raw_buffer_load_b32(src, x.vmine, ((e & 3) + 8 * (e >> 2)) * stride, 0);
+  };
+  auto place_keys = [&](const Lane& x, int buf) __attribute__((always_inline)) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) odd |= nan_bytes(held[c][e]);
-        any = __any(odd != 0);
-        if (lane == 0) odd_lds[buf][wave - 2] = any;
-      }
-      if (any) {  // wave-uniform: their keys are noted, and they enter the products as zeros
-        uint32_t* keys = odd_keys[buf][wave - 2];
-        keys[lane] = 0u;
-        keys[lane + 64] = 0u;
-        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t f = nan_bytes(held[c][e]);
-            const int t = 2 * c + (e >> 1);  // the token, in the order of the registers
-            const int key = 16 * (vgk & 1) + 4 * vhalf + (t & 3) + 8 * (t >> 2);
-#pragma unroll
-            for (int y = 0; y < 4; ++y)
-              if (f & (0x80u << (8 * y))) atomicOr(&keys[8 * vc + 4 * (e & 1) + y], 1u << key);
-            held[c][e] &= ~((f >> 7) * 0xffu);
-          }
-      }
-#pragma unroll
-      for (int hf = 0; hf < 2; ++hf) {
-        uint32_t w[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = held[e >> 1][2 * (e & 1) + hf];
-        u32x4 o[4];
-        if constexpr (decltype(f16)::value) transpose_f16(w, factor, o);
-        else transpose_bf16(w, o);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vt[buf][v_at(vgk, vhalf, 8 * vc + 4 * hf + e)] = o[e];
-      }
+    for (int c = 0; c < 2; ++c) {
+      kt[buf][k_at(x.krow, 4 * x.kpart + 2 * c)] = __builtin_bit_cast(u32x4, bf16_of(kheld[c][0], kheld[c][1]));
+      kt[buf][k_at(x.krow, 4 * x.kpart + 2 * c + 1)] = __builtin_bit_cast(u32x4, bf16_of(kheld[c][2], kheld[c][3]));
     }
+  };
+  auto put_values = [&](const Lane& x, const u32x4 (&o)[4], int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vt[buf][v_at(wave, x.half, 4 * x.li + e)] = o[e];
+  };
+  // The block of a tile's group of 16 keys.
+  auto block_of = [&](int tile, int group) __attribute__((always_inline)) {
+    return min(tile * kTile + 16 * group, len - 1) >> a.block_shift;
+  };
+  auto key_scales = [&](int tile, float (&ks)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ks[q] = scale_at(ksh, block_of(tile, q));
   };
 
   f32x16 o[4];
   float m, l;
-  uint64_t odd = 0;  // this lane's output dims that a value seen by its row makes NaN, bit 16 d + r
-
-  auto compute = [&](auto f16, int tile, int buf) __attribute__((always_inline)) {
-    constexpr bool kF16 = decltype(f16)::value;
-    const int k0 = tile * kTile;
-    // wave-uniform: nothing of the tile is seen
-    if (k0 > wmax || (k0 + kTile <= wmin - a.window + 1 && k0 >= a.sinks)) return;
-    f32x16 s[2];
+  auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+  };
+  // S^T of a tile: registers 8 i to 8 i + 7 of s[u] hold 8 of the keys 32 u + 16 i to 32 u + 16 i + 15, a block's.
+  auto scores = [&](const Lane& x, int buf, f32x16 (&s)[2]) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[u][r] = 0.f;
 #pragma unroll
-    for (int c = 0; c < 8; ++c)
+    for (int c = 0; c < 8; ++c) {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         s[u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-            __builtin_bit_cast(bf16x8, kt[buf][k_at(32 * u + li, 2 * c + half)]), __builtin_bit_cast(bf16x8, qf[c]),
+            __builtin_bit_cast(bf16x8, kt[buf][k_at(32 * u + x.li, 2 * c + x.half)]), __builtin_bit_cast(bf16x8, qf[c]),
             s[u], 0, 0, 0);
-    // Registers 8 i to 8 i + 7 of s[u] hold 8 of the keys 32 u + 16 i to 32 u + 16 i + 15, which share a block.
-    const bool all = whole && k0 + kTile - 1 <= wmin && (k0 > wmax - a.window || k0 + kTile <= a.sinks);
-    if (!all) {  // wave-uniform
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (!sees(p, k0 + 32 * u + 8 * (r / 4) + 4 * half + (r % 4), a.window, a.sinks)) s[u][r] = -INFINITY;
+      if (c & 1) __builtin_amdgcn_sched_barrier(0);  // (a few operands at a time: registers)
     }
+  };
+  auto hide = [&](const Lane& x, int p, int tile, f32x16 (&s)[2]) __attribute__((always_inline)) {
+    const int first = tile * kTile + 4 * x.half;  // key c of the lane: first + c
+    const int last = p - first, behind = p - a.window - first, sink = a.sinks - first;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int c = 32 * u + 8 * (r / 4) + (r % 4);
+        s[u][r] = (c <= last) & ((c > behind) | (c < sink)) ? s[u][r] : -INFINITY;
+      }
+  };
+  auto largest_half = [&](float mx) __attribute__((always_inline)) {  // with the row's other lane
+    const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
+  };
+  auto largest = [&](const f32x16 (&s)[2], const float (&kf)[4]) __attribute__((always_inline)) {
     float mx = -INFINITY;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
@@ -603,11 +612,10 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       for (int r = 1; r < 8; ++r) y = fmaxf(y, s[q >> 1][8 * (q & 1) + r]);
       mx = fmaxf(mx, y * kf[q]);
     }
-    {
-      const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-      mx = fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
-    }
-    // The reference moves only when a score passes it by 2^kSlack: the ratio of the sums does not depend on it.
+    return largest_half(mx);
+  };
+  // The reference moves only when a score passes it by 2^kSlack: the ratio of the sums does not depend on it.
+  auto refer = [&](float mx) __attribute__((always_inline)) {
     if (__any(mx > m + kSlack)) {  // wave-uniform
       const float mn = fmaxf(m, mx);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -618,60 +626,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= f;
     }
-    const float ref = (m == -INFINITY ? 0.f : m) - static_cast<float>(kRaise);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[u][r] = __builtin_amdgcn_exp2f(fmaf(s[u][r], kf[2 * u + (r >> 3)], -ref));
-        l += s[u][r];
-      }
-    if (!kF16 && (odd_lds[buf][0] | odd_lds[buf][1])) {  // the same for all waves
-      // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
-      // would: a hidden key's zero times NaN).
-      for (int hw = 0; hw < 2; ++hw) {
-        if (!odd_lds[buf][hw]) continue;
-        uint32_t vis = 0;
-        for (int j = 0; j < 32; ++j) vis |= sees(p, k0 + 32 * hw + j, a.window, a.sinks) ? 1u << j : 0u;
-        for (int d = 0; d < 64; ++d)
-          if (odd_keys[buf][hw][32 * (d >> 4) + 8 * ((d & 15) >> 2) + 4 * half + (d & 3)] & vis) odd |= 1ull << d;
-      }
-    }
-#pragma unroll
-    for (int gk = 0; gk < 4; ++gk) {
-      u32x4 vf[4];
-#pragma unroll
-      for (int d = 0; d < 4; ++d) vf[d] = vt[buf][v_at(gk, half, 32 * d + li)];
-      if constexpr (kF16) {
-        u32x4 part;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          part[e] = __builtin_bit_cast(
-              uint32_t, __builtin_convertvector(f32x2{s[gk >> 1][8 * (gk & 1) + 2 * e],
-                                                      s[gk >> 1][8 * (gk & 1) + 2 * e + 1]}, f16x2));
-#pragma unroll
-        for (int d = 0; d < 4; ++d)
-          o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf[d]),
-                                                        __builtin_bit_cast(f16x8, part), o[d], 0, 0, 0);
-      } else {
-        __builtin_amdgcn_sched_barrier(0);  // (one group's operands at a time: registers)
-        const float vsc = scale_at(vsh, min(k0 + 16 * gk, len - 1) >> a.block_shift);
-        u32x4 part[2];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t first, second;
-          two_parts(s[gk >> 1][8 * (gk & 1) + 2 * e] * vsc, s[gk >> 1][8 * (gk & 1) + 2 * e + 1] * vsc, first, second);
-          part[0][e] = first;
-          part[1][e] = second;
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int d = 0; d < 4; ++d)
-            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf[d]),
-                                                           __builtin_bit_cast(bf16x8, part[y]), o[d], 0, 0, 0);
-      }
-    }
+    return (m == -INFINITY ? 0.f : m) - static_cast<float>(kRaise);
   };
 
   // Whether f16 holds this workgroup's values: blocks of scales that are powers of two and near one another (those
@@ -679,7 +634,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   if (threadIdx.x < 3) vexp[threadIdx.x] = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? 255 : 0;
   __syncthreads();
   for (int i = 4 * i0 + threadIdx.x; i < 4 * i1; i += 256) {
-    const uint32_t v = __float_as_uint(vsh[min(seen.at(i >> 2) * kTile + 16 * (i & 3), len - 1) >> a.block_shift]);
+    const uint32_t v = __float_as_uint(vsh[block_of(seen.at(i >> 2), i & 3)]);
     const int e = static_cast<int>(v >> 23);
     if (v > 0x00800000u) {
       atomicMax(&vexp[0], e);
@@ -688,59 +643,271 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     }
   }
   __syncthreads();
-  const int vtop = vexp[0];
-  const bool fits = !vexp[2] && vtop < 255 && vtop - vexp[1] <= kSpread;  // the same for all
-  auto walk = [&](auto f16) __attribute__((always_inline)) {
-    // The factor of the wave's value blocks: a group of 16 keys a half wave.
-    auto factor = [&](int tile) __attribute__((always_inline)) {
-      const uint32_t v = __float_as_uint(vsh[min(tile * kTile + 16 * vgk, len - 1) >> a.block_shift]);
-      return __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(v >> 23) - vtop + 127 + kRaise, 1)) << 23);
-    };
-    float next = 1.f;
-    fetch(seen.at(i0));
-    if constexpr (decltype(f16)::value) next = factor(seen.at(i0));
-    place(f16, next, 0);
-    for (int i = i0; i < i1; ++i) {
-      const int buf = (i - i0) & 1;
-      // Tile i is in buf, and every wave is past tile i - 1 in the other one.
-      __syncthreads();
+  const int vtop = __builtin_amdgcn_readfirstlane(vexp[0]);
+  const bool fits = !__builtin_amdgcn_readfirstlane(vexp[2]) && vtop < 255 &&
+                    vtop - __builtin_amdgcn_readfirstlane(vexp[1]) <= kSpread;  // the same for all
+
+  // A value block's factor on its way to f16.
+  auto value_factor = [&](float scale) __attribute__((always_inline)) {
+    const uint32_t v = __float_as_uint(scale);
+    return __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(v >> 23) - vtop + 127 + kRaise, 1)) << 23);
+  };
+
+  auto place_f16 = [&](const Lane& x, int tile, int buf) __attribute__((always_inline)) {
+    u32x4 o4[4];
+    const float factor = value_factor(scale_at(vsh, block_of(tile, wave)));
 #pragma unroll
-      for (int q = 0; q < 4; ++q) kf[q] = kn[q];
-      if (i + 1 < i1) {
-        fetch(seen.at(i + 1));
-        if constexpr (decltype(f16)::value) next = factor(seen.at(i + 1));
+    for (int y = 0; y < 2; ++y)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        f16_pair(vheld[2 * e], vheld[2 * e + 1], factor, y, e, o4[2 * y], o4[2 * y + 1]);
+    put_values(x, o4, buf);
+  };
+
+  // Tiles that every row sees whole, values and probabilities in f16, one product. Tile i's probabilities and their product are taken
+  // while tile i + 1's scores are, tile i + 2's keys and i + 1's values go to LDS and the next ones are on their way:
+  // one barrier a tile, and vector work beside every matrix instruction. The order is written down slice by slice (a
+  // scheduler of its own would read all operands first, and spill).
+  auto walk_whole = [&](int from, int to) __attribute__((always_inline)) {
+    if (from >= to) return;  // workgroup-uniform
+    __syncthreads();         // every wave is past the tiles before these
+    const Lane g = own_lane();
+    int kbase = k_at(g.li, g.half);
+    const int end = to - 1;
+    auto tile_at = [&](int i) __attribute__((always_inline)) { return seen.at(min(i, end)); };
+    // Scales of a tile's groups of 16 keys, a tile ahead, in a lane each: the keys' in lanes 0 to 3, the values' in 4 to 7.
+    float held_scales[3];
+    auto fetch_scales = [&](int tile) __attribute__((always_inline)) {
+      return (g.li & 4 ? vsh : ksh)[block_of(tile, g.li & 3)];
+    };
+    auto lane_scale = [&](float held, int which) __attribute__((always_inline)) {
+      return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), which));
+    };
+    // One tile: its scores in s, the next one's into sn (past the last, the last one's again). Keys i are in kt[par],
+    // values in vt[par]. 32 slices of a matrix instruction each (16 of the next scores, 16 of this product), its
+    // operand read from LDS three slices before.
+    auto step = [&](auto par_, int i, f32x16 (&s)[2], f32x16 (&sn)[2]) __attribute__((always_inline)) {
+      constexpr int par = decltype(par_)::value;
+      // Every wave is past tile i - 1's values and tile i's keys; tile i's values and tile i + 1's keys are in place.
+      barrier_lds();
+      asm volatile("" : "+v"(kbase));  // (its eight forms are made anew each time: registers)
+      u32x4 f[4];
+      auto operand = [&](int j) __attribute__((always_inline)) {
+        if (j < 16) f[j & 3] = kt[par ^ 1][512 * (j & 1) + (kbase ^ (j & 14))];  // k_at(32 u + li, 2 c + half)
+        else f[j & 3] = vt[par][v_at((j - 16) >> 2, g.half, 32 * (j & 3) + g.li)];
+      };
+#pragma unroll
+      for (int j = 0; j < 3; ++j) operand(j);
+      float kf[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) kf[q] = key_factor(lane_scale(held_scales[0], q), a.scale_log2e);
+      const float factor = value_factor(lane_scale(held_scales[1], 4 + wave));
+      float mx = -INFINITY, ref = 0.f;
+      auto largest_of = [&](int q) __attribute__((always_inline)) {
+        mx = fmaxf(mx, max8(s[q >> 1], 8 * (q & 1)) * kf[q]);
+      };
+      u32x4 part[4];
+      auto probabilities = [&](int gk, int e) __attribute__((always_inline)) {
+        const float x0 = __builtin_amdgcn_exp2f(fmaf(s[gk >> 1][8 * (gk & 1) + 2 * e], kf[gk], -ref));
+        const float x1 = __builtin_amdgcn_exp2f(fmaf(s[gk >> 1][8 * (gk & 1) + 2 * e + 1], kf[gk], -ref));
+        const f16x2 x = __builtin_convertvector(f32x2{x0, x1}, f16x2);
+        l = __builtin_amdgcn_fdot2(x, f16x2{1, 1}, l, false);  // (the sum of what the product takes)
+        part[gk][e] = __builtin_bit_cast(uint32_t, x);
+      };
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) sn[u][r] = 0.f;
+      u32x4 x[2];
+      largest_of(0);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) {
+        if (j < 29) operand(j + 3);
+        if (j < 16)
+          sn[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[j & 3]),
+                                                              __builtin_bit_cast(bf16x8, qf[j >> 1]), sn[j & 1], 0, 0, 0);
+        else
+          o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f[j & 3]),
+                                                            __builtin_bit_cast(f16x8, part[(j - 16) >> 2]), o[j & 3], 0,
+                                                            0, 0);
+        if (j < 3) largest_of(j + 1);
+        else if (j == 3) ref = refer(largest_half(mx));
+        else if (j < 20) probabilities((j - 4) >> 2, j & 3);
+        else if (j < 24) {
+          const int c = j - 20;
+          kt[par][k_at(g.krow, 4 * g.kpart + c)] = __builtin_bit_cast(
+              u32x4, bf16_of(kheld[c >> 1][2 * (c & 1)], kheld[c >> 1][2 * (c & 1) + 1]));
+        } else if (j < 28) {  // two tokens' pairs of two dims
+          const int y = (j - 24) >> 1;
+#pragma unroll
+          for (int e = 2 * (j & 1); e < 2 * (j & 1) + 2; ++e)
+            f16_pair(vheld[2 * e], vheld[2 * e + 1], factor, y, e, x[0], x[1]);
+          if (j & 1)
+#pragma unroll
+            for (int z = 0; z < 2; ++z) vt[par ^ 1][v_at(wave, g.half, 4 * g.li + 2 * y + z)] = x[z];
+        } else if (j == 28) {
+          fetch_keys(g, tile_at(i + 3));
+        } else if (j == 29) {
+          fetch_values(g, tile_at(i + 2));
+        } else if (j == 30) {
+          held_scales[0] = held_scales[1];
+          held_scales[1] = held_scales[2];
+          held_scales[2] = fetch_scales(tile_at(i + 3));
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      compute(f16, seen.at(i), buf);
-      if (i + 1 < i1) place(f16, next, buf ^ 1);
+    };
+    fetch_keys(g, tile_at(from));
+    fetch_values(g, tile_at(from));
+    place_keys(g, 0);
+    place_f16(g, tile_at(from), 0);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_keys(g, tile_at(from + 1));
+    place_keys(g, 1);
+    __builtin_amdgcn_sched_barrier(0);
+    fetch_keys(g, tile_at(from + 2));
+    fetch_values(g, tile_at(from + 1));
+    __syncthreads();
+    f32x16 sa[2], sb[2];
+    scores(g, 0, sa);
+#pragma unroll
+    for (int t = 0; t < 3; ++t) held_scales[t] = fetch_scales(tile_at(from + t));
+    for (int i = from;;) {
+      step(std::integral_constant<int, 0>{}, i, sa, sb);
+      if (++i > end) break;
+      step(std::integral_constant<int, 1>{}, i, sb, sa);
+      if (++i > end) break;
     }
   };
-  auto clear = [&]() __attribute__((always_inline)) {
+
+  // Any tiles, one after the other: f16 as above, or for any values bf16, two parts of a probability times its block's
+  // scale, and NaN kept to the rows that see them.
+  uint64_t odd = 0;  // this lane's output dims that a value seen by its row makes NaN, bit 16 d + r
+  auto place_any = [&](const Lane& x, int buf) __attribute__((always_inline)) {
+    uint32_t some = 0;
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
+    for (int e = 0; e < 8; ++e) some |= nan_bytes(vheld[e]);
+    const bool any = __any(some != 0);
+    if (lane == 0) odd_lds[buf][wave] = any;
+    if (any) {  // wave-uniform: their keys are noted, and they enter the products as zeros
+      uint32_t* keys = odd_keys[buf][wave];
+      keys[lane] = 0u;
+      keys[lane + 64] = 0u;
+      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
 #pragma unroll
-      for (int r = 0; r < 16; ++r) o[d][r] = 0.f;
-    m = -INFINITY;
-    l = 0.f;
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t f = nan_bytes(vheld[e]);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (f & (0x80u << (8 * y))) atomicOr(&keys[4 * x.li + y], 1u << (4 * x.half + (e & 3) + 8 * (e >> 2)));
+        vheld[e] &= ~((f >> 7) * 0xffu);
+      }
+    }
+    u32x4 o4[4];
+    transpose_bf16(vheld, o4);
+    put_values(x, o4, buf);
   };
+  auto walk = [&](auto f16, int from, int to) __attribute__((always_inline)) {
+    constexpr bool kF16 = decltype(f16)::value;
+    if (from >= to) return;  // workgroup-uniform
+    const Lane g = own_lane();
+    const Row mine = row_of(g.li);
+    const int p = mine.query ? p0 + mine.t : pmax;
+    __syncthreads();  // every wave is past the tiles before these
+    fetch_keys(g, seen.at(from));
+    fetch_values(g, seen.at(from));
+    for (int i = from; i < to; ++i) {
+      const int buf = (i - from) & 1, tile = seen.at(i);
+      place_keys(g, buf);
+      if constexpr (kF16) place_f16(g, tile, buf);
+      else place_any(g, buf);
+      __syncthreads();  // (and every wave is past the tile before last, whose place the next one takes)
+      if (i + 1 < to) {
+        fetch_keys(g, seen.at(i + 1));
+        fetch_values(g, seen.at(i + 1));
+      }
+      f32x16 s[2];
+      float kf[4];
+      scores(g, buf, s);
+      key_scales(tile, kf);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) kf[q] = key_factor(kf[q], a.scale_log2e);
+      hide(g, p, tile, s);
+      const float ref = refer(largest(s, kf));
+      if constexpr (!kF16) {
+        for (int q = 0; q < 4; ++q) {
+          // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
+          // would: a hidden key's zero times NaN).
+          if (!odd_lds[buf][q]) continue;  // the same for all
+          uint32_t vis = 0;
+          for (int j = 0; j < 16; ++j) vis |= sees(p, tile * kTile + 16 * q + j, a.window, a.sinks) ? 1u << j : 0u;
+          for (int d = 0; d < 64; ++d)
+            if (odd_keys[buf][q][32 * (d >> 4) + 8 * ((d & 15) >> 2) + 4 * g.half + (d & 3)] & vis) odd |= 1ull << d;
+        }
+      }
+#pragma unroll
+      for (int gk = 0; gk < 4; ++gk) {
+        __builtin_amdgcn_sched_barrier(0);  // (one group's operands at a time: registers)
+        const float vsc = kF16 ? 1.f : scale_at(vsh, block_of(tile, gk));
+        u32x4 part[2];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x0 = __builtin_amdgcn_exp2f(fmaf(s[gk >> 1][8 * (gk & 1) + 2 * e], kf[gk], -ref));
+          const float x1 = __builtin_amdgcn_exp2f(fmaf(s[gk >> 1][8 * (gk & 1) + 2 * e + 1], kf[gk], -ref));
+          if constexpr (kF16) {
+            const f16x2 x = __builtin_convertvector(f32x2{x0, x1}, f16x2);
+            l = __builtin_amdgcn_fdot2(x, f16x2{1, 1}, l, false);  // (the sum of what the product takes)
+            part[0][e] = __builtin_bit_cast(uint32_t, x);
+          } else {
+            l += x0 + x1;
+            uint32_t first, second;
+            two_parts(x0 * vsc, x1 * vsc, first, second);
+            part[0][e] = first;
+            part[1][e] = second;
+          }
+        }
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {
+          const u32x4 vf = vt[buf][v_at(gk, g.half, 32 * d + g.li)];
+          if constexpr (kF16) {
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, vf),
+                                                          __builtin_bit_cast(f16x8, part[0]), o[d], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+              o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, vf),
+                                                             __builtin_bit_cast(bf16x8, part[y]), o[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+  };
+
+  // Of tiles i0 to i1 - 1 those that every row sees whole: j0 to j1 - 1.
+  const int low = a.window < kNoWindow ? max(0, pmax - a.window + kTile) >> kTileShift : 0;
+  const int j0 = min(max(seen.index(low), i0), i1), j1 = min(max(seen.index((pmin + 1) >> kTileShift), j0), i1);
   clear();
   float back = 1.f;  // what the values' sums are multiplied with in the end
   if (i0 < i1) {     // workgroup-uniform
     bool exact = fits;
     if (fits) {
-      walk(std::true_type{});
+      walk(std::true_type{}, i0, j0);
+      walk_whole(j0, j1);
+      walk(std::true_type{}, j1, i1);
       back = __builtin_ldexpf(1.f, vtop - 127 - kRaise);
       // NaN anywhere: a value may have reached rows that do not see it.
-      bool odd = false;
+      bool nan = false;
 #pragma unroll
       for (int d = 0; d < 4; ++d)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) odd |= o[d][r] != o[d][r];
-      exact = !__syncthreads_or(odd);
+        for (int r = 0; r < 16; ++r) nan |= o[d][r] != o[d][r];
+      exact = !__syncthreads_or(nan);
     }
     if (!exact) {
       clear();
       back = 1.f;
-      walk(std::false_type{});
+      walk(std::false_type{}, i0, i1);
     }
   }
 
@@ -748,14 +915,17 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(l), __float_as_uint(l), false, false);
     l = __uint_as_float(w[0]) + __uint_as_float(w[1]);
   }
-  if (row >= R) return;
+  const Lane g = own_lane();
+  const Row x = row_of(g.li);
+  if (x.row >= R) return;
+  if (!x.query) back = l = 0.f;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
     for (int r = 0; r < 16; ++r) o[d][r] = (odd >> (16 * d + r)) & 1 ? __builtin_nanf("") : o[d][r] * back;
   if (a.splits == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // (nothing seen: zeros)
-    uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H * G + h * G + g) * kD + 4 * half;
+    uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + x.t) * a.H * G + h * G + x.g) * kD + 4 * g.half;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
@@ -764,12 +934,12 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
                                                            skv::f2bf2(o[d][4 * r + 2] * inv, o[d][4 * r + 3] * inv)};
     return;
   }
-  const int64_t at = (static_cast<int64_t>(bh) * R + row) * a.splits + split;
-  if (half == 0) {
+  const int64_t at = (static_cast<int64_t>(bh) * R + x.row) * a.splits + split;
+  if (g.half == 0) {
     a.ws_ml[2 * at] = m;
     a.ws_ml[2 * at + 1] = l;
   }
-  float* dst = a.ws_o + at * kD + 4 * half;
+  float* dst = a.ws_o + at * kD + 4 * g.half;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
