@@ -415,7 +415,7 @@ constexpr int kRowsTile = 4 * kRowsWave;
 
 // 16-byte chunk c (8 dims) of key row r of a tile in LDS, and chunk (group of 16 keys, half of its order, dim).
 __device__ __forceinline__ int k_at(int r, int c) { return r * 16 + (c ^ (r & 15)); }
-__device__ __forceinline__ int v_at(int gk, int half, int d) { return gk * 256 + half * 128 + (d ^ ((d >> 3) & 7)); }
+__device__ __forceinline__ int v_at(int gk, int half, int d) { return gk * 256 + half * 128 + (d ^ ((d >> 4) & 3)); }
 
 __device__ __forceinline__ u32x4 load4(const uint8_t* p) { return *reinterpret_cast<const u32x4*>(p); }
 
@@ -918,11 +918,14 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   const Lane g = own_lane();
   const Row x = row_of(g.li);
   if (x.row >= R) return;
-  if (!x.query) back = l = 0.f;
+  if (!x.query) l = 0.f;
 #pragma unroll
   for (int d = 0; d < 4; ++d)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) o[d][r] = (odd >> (16 * d + r)) & 1 ? __builtin_nanf("") : o[d][r] * back;
+    for (int r = 0; r < 16; ++r) {
+      const float v = (odd >> (16 * d + r)) & 1 ? __builtin_nanf("") : o[d][r] * back;
+      o[d][r] = x.query ? v : 0.f;
+    }
   if (a.splits == 1) {
     const float inv = l == 0.f ? 0.f : 1.f / l;  // (nothing seen: zeros)
     uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + x.t) * a.H * G + h * G + x.g) * kD + 4 * g.half;

@@ -364,6 +364,24 @@ def test_attn_nan_where_seen_and_hidden(gpu, T):
         assert torch.equal(got[1, :, 4:].isnan().any(-1), see.unsqueeze(1).expand(T, 4))
 
 
+@pytest.mark.parametrize("T", [3, 45])
+def test_attn_padding_beside_nan(gpu, T):
+    """Padding rows are zeros where the sequence's own rows are NaN, and where their queries are NaN or infinite."""
+    _say(f"kv8_attn padding beside NaN T={T}")
+    g = torch.Generator().manual_seed(T)
+    caches = _filled(2, 2, 128, 32, g, gpu)
+    caches[1].view(torch.uint8)[:, :, 60] = 0x7f
+    q = _queries(2, 8, T, g, gpu)
+    q[:, :, T - 1] = math.nan
+    q[0, :, T - 1] = math.inf
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    got = shadowkv.kv8_attn(q, *caches, ints([100, 61]), counts=ints([T - 1, 1]), block=32)
+    sees = _see(T - 1, T, 100, None, 0)[:T - 1, 60].to(gpu)  # (the last queries of the 99 positions before)
+    assert torch.equal(got[0, :T - 1].isnan().all(-1), sees.unsqueeze(1).expand(-1, 8)) and got[1, :1].isnan().all()
+    assert not got[0, :T - 1][~sees].isnan().any()
+    assert (got[0, T - 1:] == 0).all() and (got[1, 1:] == 0).all()
+
+
 @pytest.mark.parametrize("T", [1, 40])
 def test_attn_scores_of_every_size(gpu, T):
     """Scores that grow along the keys (the running maximum moves in every tile), that fall, and all-equal ones;
