@@ -47,9 +47,9 @@ struct Args {
   int B, H, G, T, cap, block_shift, window, sinks;
   float scale_log2e;  // of the scale's magnitude
   bool negative;      // whether the scale is: the queries' sign is turned instead
-  int target;   // one token: workgroups to aim for
-  int splits;   // many: shares of a row tile's keys
-  int rtiles;   // many: row tiles of a (sequence, kv head)
+  int target;   // few rows: workgroups to aim for
+  int splits;   // more: shares of a row tile's keys
+  int rtiles;   // more: row tiles of a (sequence, kv head)
 };
 
 __device__ __forceinline__ int length_of(const Args& a, int b) { return min(max(a.lengths[b], 0), a.cap); }
@@ -141,12 +141,12 @@ __device__ __forceinline__ float sum_of_rows(float x) {
 }
 
 // ------------------------------------------------------------------------------------------------
-// One new token a sequence, at most 16 query heads to a kv head.
+// Few rows: up to 32 of a kv head's query heads and new tokens together (row t * G + g).
 //
 // Bound: HBM, 256 bytes a key. The sequences' keys are cut into chunks of equal length, however different the
 // sequences are (planned on the device from the lengths, so that a captured call follows them), each a workgroup
 // of four waves that take its groups of 32 keys in turn, straight from memory into registers: S^T = K Q^T on
-// v_mfma_f32_16x16x32_bf16 (a query head a column) leaves a lane with 8 keys' scores of one head, which is the
+// v_mfma_f32_16x16x32_bf16 (a row of the queries a column) leaves a lane with 8 keys' scores of one row, which is the
 // second operand of O^T = V^T P^T, whose first is the lane's 8 tokens of one dim: neither probabilities nor
 // values cross lanes.
 constexpr int kGroup = 32;
@@ -159,16 +159,16 @@ struct Chunk {
   int b, index, groups;  // sequence, which of its chunks, groups of a chunk
 };
 
-__device__ __forceinline__ Groups token_groups(const Args& a, int b) {
-  const int p = length_of(a, b) - 1;
-  return groups_seen(count_of(a, b) ? p : -1, count_of(a, b) ? p : -1, a.window, a.sinks, kGroupShift);
+__device__ __forceinline__ Groups few_groups(const Args& a, int b) {
+  const int len = length_of(a, b), n = count_of(a, b);
+  return groups_seen(len - n, n ? len - 1 : -1, a.window, a.sinks, kGroupShift);
 }
 
 // The chunk length, wave-uniform: the sequences' groups dealt over the workgroups to aim for.
 __device__ __forceinline__ int chunk_groups(const Args& a, int lane) {
   int64_t total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int t = b0 + lane < a.B ? token_groups(a, b0 + lane).total : 0;
+    const int t = b0 + lane < a.B ? few_groups(a, b0 + lane).total : 0;
     total += __builtin_amdgcn_readlane(skv::wave_inclusive_scan(t), 63);
   }
   return static_cast<int>(max(static_cast<int64_t>(kMinGroups), (total * a.H + a.target - 1) / a.target));
@@ -179,7 +179,7 @@ __device__ __forceinline__ bool find_chunk(const Args& a, int i, int lane, Chunk
   c.groups = chunk_groups(a, lane);
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = b0 + lane < a.B ? (token_groups(a, b0 + lane).total + c.groups - 1) / c.groups : 0;
+    const int n = b0 + lane < a.B ? (few_groups(a, b0 + lane).total + c.groups - 1) / c.groups : 0;
     const int incl = before + skv::wave_inclusive_scan(n);
     const uint64_t hit = __ballot(i < incl && i >= incl - n);
     if (hit) {
@@ -193,7 +193,11 @@ __device__ __forceinline__ bool find_chunk(const Args& a, int i, int lane, Chunk
   return false;
 }
 
-__global__ void __launch_bounds__(256) token_kernel(Args a) {
+// 0x80 in each byte that is a NaN code.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+template <int kTiles>  // of 16 rows
+__global__ void __launch_bounds__(256, kTiles == 1 ? 4 : 2) few_kernel(Args a) {
   __shared__ float o_lds[4][16][kOutLd];
   __shared__ float m_lds[4][16], l_lds[4][16];
   const int lane = threadIdx.x & 63;
@@ -201,30 +205,41 @@ __global__ void __launch_bounds__(256) token_kernel(Args a) {
   const int slot = blockIdx.x / a.H, h = blockIdx.x - slot * a.H;
   Chunk c;
   if (!find_chunk(a, slot, lane, c)) return;  // workgroup-uniform
-  const int b = c.b, G = a.G;
-  const int len = length_of(a, b), p = len - 1;
-  const Groups seen = token_groups(a, b);
+  const int b = c.b, G = a.G, R = G * a.T;
+  const int len = length_of(a, b), n = count_of(a, b);
+  const int pmin = len - n, pmax = len - 1;
+  const Groups seen = few_groups(a, b);
   const int i0 = c.index * c.groups, i1 = min(i0 + c.groups, seen.total);
   const int li = lane & 15, grp = lane >> 4;
 
-  // Q as the B operand: lane (li, grp) holds head li, in step s dims 64 (s / 2) + 16 grp + 8 (s % 2) and on.
-  bf16x8 qf[4];
-  {
-    const uint16_t* q = a.q + b * a.q_sb + (h * G + min(li, G - 1)) * a.q_sh + 16 * grp;
+  // Q as the B operand: lane (li, grp) holds row li of a tile, in step s dims 64 (s / 2) + 16 grp + 8 (s % 2) and on.
+  // Rows past the last, and of padding, ride along with the last query, and give nothing in the end.
+  bf16x8 qf[kTiles][4];
+  int p[kTiles];
+#pragma unroll
+  for (int y = 0; y < kTiles; ++y) {
+    const int row = min(16 * y + li, R - 1), t = row / G;
+    p[y] = t < n ? pmin + t : pmax;
+    const uint16_t* q = a.q + b * a.q_sb + (h * G + row - t * G) * a.q_sh + t * a.q_st + 16 * grp;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
-      qf[s] = __builtin_bit_cast(bf16x8, skv::load16_or_zero(q + 64 * (s >> 1) + 8 * (s & 1), li < G) ^
-                                             (a.negative ? 0x80008000u : 0u));
+      qf[y][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 64 * (s >> 1) + 8 * (s & 1)) ^
+                                                (a.negative ? 0x80008000u : 0u));
   }
   const uint8_t* kh = a.k8 + b * a.c_sb + h * a.c_sh + 16 * grp;
   const uint8_t* vh = a.v8 + b * a.c_sb + h * a.c_sh + 8 * li;
   const float* ksh = a.ks + b * a.s_sb + h * a.s_sh;
   const float* vsh = a.vs + b * a.s_sb + h * a.s_sh;
 
-  f32x4 o[8];
+  f32x4 o[kTiles][8];
+  float m[kTiles], l[kTiles];  // the row's reference, in units of log2; this lane's share of its sum
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;  // the head's reference, in units of log2; this lane's share of its sum
+  for (int y = 0; y < kTiles; ++y) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[y][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m[y] = -INFINITY;
+    l[y] = 0.f;
+  }
 
   u32x4 kr[2][2];
   u32x2 vr[8];
@@ -233,10 +248,10 @@ __global__ void __launch_bounds__(256) token_kernel(Args a) {
     const int j0 = seen.at(i) * kGroup;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const uint8_t* row = kh + static_cast<int64_t>(min(j0 + 16 * u + li, p)) * a.c_ss;
+      const uint8_t* row = kh + static_cast<int64_t>(min(j0 + 16 * u + li, pmax)) * a.c_ss;
       kr[u][0] = *reinterpret_cast<const u32x4*>(row);
       kr[u][1] = *reinterpret_cast<const u32x4*>(row + 64);
-      const int blk = min(j0 + 16 * u, p) >> a.block_shift;
+      const int blk = min(j0 + 16 * u, pmax) >> a.block_shift;
       kc[u] = ksh[blk];
       vc[u] = vsh[blk];
     }
@@ -245,59 +260,111 @@ __global__ void __launch_bounds__(256) token_kernel(Args a) {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         vr[4 * u + r] = *reinterpret_cast<const u32x2*>(
-            vh + static_cast<int64_t>(min(j0 + 16 * u + 4 * grp + r, p)) * a.c_ss);
+            vh + static_cast<int64_t>(min(j0 + 16 * u + 4 * grp + r, pmax)) * a.c_ss);
   };
 
   for (int i = i0 + wave; i < i1; i += 4) {
     load(i);
     const int j0 = seen.at(i) * kGroup;
-    f32x4 s[2];
+    f32x4 s[kTiles][2];
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < 4; ++st)
-        s[u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            bf16_of(kr[u][st >> 1][2 * (st & 1)], kr[u][st >> 1][2 * (st & 1) + 1]), qf[st], s[u], 0, 0, 0);
       const float f = key_factor(kc[u], a.scale_log2e);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) s[u][r] *= f;
+      for (int y = 0; y < kTiles; ++y) s[y][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < 4; ++st) {
+        const bf16x8 kf = bf16_of(kr[u][st >> 1][2 * (st & 1)], kr[u][st >> 1][2 * (st & 1) + 1]);
+#pragma unroll
+        for (int y = 0; y < kTiles; ++y)
+          s[y][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, qf[y][st], s[y][u], 0, 0, 0);
+      }
+#pragma unroll
+      for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s[y][u][r] *= f;
     }
-    // wave-uniform: a group at an end of what the token sees. Hidden values may be anything: zero codes.
-    if (j0 + kGroup > len || (j0 < len - a.window && j0 + kGroup > a.sinks)) {
+    // wave-uniform: a group at an end of what a row sees
+    if (j0 + kGroup > pmin + 1 || (j0 <= pmax - a.window && j0 + kGroup > a.sinks)) {
+      uint32_t odd = 0;
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (!sees(p, j0 + 16 * u + 4 * grp + r, a.window, a.sinks)) {
-            s[u][r] = -INFINITY;
-            vr[4 * u + r] = u32x2{0u, 0u};
+        for (int r = 0; r < 4; ++r) {
+          const int j = j0 + 16 * u + 4 * grp + r;
+#pragma unroll
+          for (int y = 0; y < kTiles; ++y)
+            if (!sees(p[y], j, a.window, a.sinks)) s[y][u][r] = -INFINITY;
+          // a value that no row sees may be anything: zero codes
+          u32x2& w = vr[4 * u + r];
+          if (!(j <= pmax && (j > pmin - a.window || j < a.sinks))) w = u32x2{0u, 0u};
+          odd |= nan_bytes(w[0]) | nan_bytes(w[1]);
+        }
+      if (n > 1 && __any(odd != 0)) {  // wave-uniform
+        // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
+        // would: a hidden key's zero times NaN): how many such keys a row sees is a product of its own.
+        uint32_t ones[2][8];
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t f = nan_bytes(vr[t][x]) >> 7;
+            ones[x][t] = f * 0x38u;  // 1
+            vr[t][x] &= ~(f * 0xffu);
           }
-    }
-    float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[0][2], s[0][3])),
-                     fmaxf(fmaxf(s[1][0], s[1][1]), fmaxf(s[1][2], s[1][3])));
-    mx = max_of_rows(mx);
-    if (__any(mx > m)) {  // wave-uniform
-      const float mn = fmaxf(m, mx);
-      const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) o[e] *= f;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;
-    u32x4 part[2];
+        for (int y = 0; y < kTiles; ++y) {
+          u32x4 vis;
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
+          for (int e = 0; e < 4; ++e) {
+            const int j = j0 + 16 * (e >> 1) + 4 * grp + 2 * (e & 1);
+            vis[e] = (sees(p[y], j, a.window, a.sinks) ? 0x3f80u : 0u) |
+                     (sees(p[y], j + 1, a.window, a.sinks) ? 0x3f800000u : 0u);
+          }
 #pragma unroll
-      for (int r = 0; r < 4; r += 2) {
-        const float p0 = __builtin_amdgcn_exp2f(s[u][r] - ref), p1 = __builtin_amdgcn_exp2f(s[u][r + 1] - ref);
-        l += p0 + p1;
-        uint32_t first, second;
-        two_parts(p0 * vc[u], p1 * vc[u], first, second);
-        part[0][2 * u + r / 2] = first;
-        part[1][2 * u + r / 2] = second;
+          for (int x = 0; x < 2; ++x) {
+            u32x4 is[4];
+            transpose_bf16(ones[x], is);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              f32x4 count = {0.f, 0.f, 0.f, 0.f};
+              count = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, is[e]),
+                                                              __builtin_bit_cast(bf16x8, vis), count, 0, 0, 0);
+#pragma unroll
+              for (int r = 0; r < 4; ++r)
+                if (count[r] > 0.f) o[y][4 * x + e][r] = __builtin_nanf("");
+            }
+          }
+        }
       }
+    }
+    u32x4 part[kTiles][2];
+#pragma unroll
+    for (int y = 0; y < kTiles; ++y) {
+      float mx = fmaxf(fmaxf(fmaxf(s[y][0][0], s[y][0][1]), fmaxf(s[y][0][2], s[y][0][3])),
+                       fmaxf(fmaxf(s[y][1][0], s[y][1][1]), fmaxf(s[y][1][2], s[y][1][3])));
+      mx = max_of_rows(mx);
+      if (__any(mx > m[y])) {  // wave-uniform
+        const float mn = fmaxf(m[y], mx);
+        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[y] - mn);
+        m[y] = mn;
+        l[y] *= f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[y][e] *= f;
+      }
+      const float ref = m[y] == -INFINITY ? 0.f : m[y];
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int r = 0; r < 4; r += 2) {
+          const float p0 = __builtin_amdgcn_exp2f(s[y][u][r] - ref), p1 = __builtin_amdgcn_exp2f(s[y][u][r + 1] - ref);
+          l[y] += p0 + p1;
+          uint32_t first, second;
+          two_parts(p0 * vc[u], p1 * vc[u], first, second);
+          part[y][0][2 * u + r / 2] = first;
+          part[y][1][2 * u + r / 2] = second;
+        }
+    }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t w[8];
@@ -309,45 +376,54 @@ __global__ void __launch_bounds__(256) token_kernel(Args a) {
       for (int e = 0; e < 4; ++e)
 #pragma unroll
         for (int x = 0; x < 2; ++x)
-          o[4 * half + e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              __builtin_bit_cast(bf16x8, vf[e]), __builtin_bit_cast(bf16x8, part[x]), o[4 * half + e], 0, 0, 0);
+#pragma unroll
+          for (int y = 0; y < kTiles; ++y)
+            o[y][4 * half + e] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[e]),
+                                                        __builtin_bit_cast(bf16x8, part[y][x]), o[y][4 * half + e], 0, 0, 0);
     }
   }
 
-  // The waves' parts: lane (li, grp) holds head li's dims 8 (4 grp + r) + e.
-  l = sum_of_rows(l);
-  if (grp == 0) {
-    m_lds[wave][li] = m;
-    l_lds[wave][li] = l;
-  }
-  if (li < G) {
+  // The waves' parts: lane (li, grp) holds row li's dims 8 (4 grp + r) + e.
+  const int64_t row0 = (static_cast<int64_t>(slot) * a.H + h) * R;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-      for (int e = 0; e < 8; e += 4)
-        *reinterpret_cast<f32x4*>(&o_lds[wave][li][8 * (4 * grp + r) + e]) =
-            f32x4{o[e][r], o[e + 1][r], o[e + 2][r], o[e + 3][r]};
-  }
-  __syncthreads();
-  const int64_t row0 = (static_cast<int64_t>(slot) * a.H + h) * G;
-  for (int i = threadIdx.x; i < G * 32; i += 256) {
-    const int g = i >> 5, d = 4 * (i & 31);
-    float top = m_lds[0][g];
-#pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][g]);
-    const float ref = top == -INFINITY ? 0.f : top;
-    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
-    float ls = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float f = __builtin_amdgcn_exp2f(m_lds[w][g] - ref);
-      ls += f * l_lds[w][g];
-      sum += f * *reinterpret_cast<const f32x4*>(&o_lds[w][g][d]);
+  for (int y = 0; y < kTiles; ++y) {
+    const float ls = sum_of_rows(l[y]);
+    const int rows = min(16, R - 16 * y);
+    if (y) __syncthreads();
+    if (grp == 0) {
+      m_lds[wave][li] = m[y];
+      l_lds[wave][li] = ls;
     }
-    *reinterpret_cast<f32x4*>(a.ws_o + (row0 + g) * kD + d) = sum;
-    if (d == 0) {
-      a.ws_ml[2 * (row0 + g)] = top;
-      a.ws_ml[2 * (row0 + g) + 1] = ls;
+    if (li < rows) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int e = 0; e < 8; e += 4)
+          *reinterpret_cast<f32x4*>(&o_lds[wave][li][8 * (4 * grp + r) + e]) =
+              f32x4{o[y][e][r], o[y][e + 1][r], o[y][e + 2][r], o[y][e + 3][r]};
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < rows * 32; i += 256) {
+      const int g = i >> 5, d = 4 * (i & 31), row = 16 * y + g;
+      const bool query = row / G < n;  // (padding: as if it had seen nothing)
+      float top = m_lds[0][g];
+#pragma unroll
+      for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][g]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      float lsum = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float f = __builtin_amdgcn_exp2f(m_lds[w][g] - ref);
+        lsum += f * l_lds[w][g];
+        sum += f * *reinterpret_cast<const f32x4*>(&o_lds[w][g][d]);
+      }
+      *reinterpret_cast<f32x4*>(a.ws_o + (row0 + row) * kD + d) = query ? sum : f32x4{0.f, 0.f, 0.f, 0.f};
+      if (d == 0) {
+        a.ws_ml[2 * (row0 + row)] = query ? top : -INFINITY;
+        a.ws_ml[2 * (row0 + row) + 1] = query ? lsum : 0.f;
+      }
     }
   }
 }
@@ -383,25 +459,25 @@ __device__ __forceinline__ void join_parts(const float* ws_o, const float* ws_ml
   }
 }
 
-__global__ void __launch_bounds__(256) token_join_kernel(Args a) {
+__global__ void __launch_bounds__(256) few_join_kernel(Args a) {
   __shared__ f32x4 acc_lds[8][32];
   const int lane = threadIdx.x & 63;
-  const int Hq = a.H * a.G;
-  const int b = blockIdx.x / Hq, hq = blockIdx.x - b * Hq;
-  const int h = hq / a.G, g = hq - h * a.G;
+  const int Hq = a.H * a.G, bt = blockIdx.x / Hq, hq = blockIdx.x - bt * Hq;
+  const int b = bt / a.T, t = bt - b * a.T, h = hq / a.G, g = hq - h * a.G;
   const int each = chunk_groups(a, lane);
   int before = 0;
   for (int b0 = 0; b0 < b; b0 += 64) {
-    const int n = b0 + lane < b ? (token_groups(a, b0 + lane).total + each - 1) / each : 0;
+    const int n = b0 + lane < b ? (few_groups(a, b0 + lane).total + each - 1) / each : 0;
     before += __builtin_amdgcn_readlane(skv::wave_inclusive_scan(n), 63);
   }
-  const int n = (token_groups(a, b).total + each - 1) / each;
-  join_parts(a.ws_o, a.ws_ml, (static_cast<int64_t>(before) * a.H + h) * a.G + g, static_cast<int64_t>(a.H) * a.G, n,
+  const int n = (few_groups(a, b).total + each - 1) / each;
+  const int64_t R = static_cast<int64_t>(a.T) * a.G;
+  join_parts(a.ws_o, a.ws_ml, (static_cast<int64_t>(before) * a.H + h) * R + t * a.G + g, a.H * R, n,
              a.out + static_cast<int64_t>(blockIdx.x) * kD, acc_lds);
 }
 
 // ------------------------------------------------------------------------------------------------
-// Several new tokens a sequence, or more than 16 query heads to a kv head.
+// More rows.
 //
 // Bound: the matrix cores (with few rows, HBM). The rows of a kv head are its queries' heads together, row
 // t * G + g, so that a tile of keys serves all of them. A workgroup of four waves owns 128 rows (32 a wave, a row
@@ -436,9 +512,6 @@ __device__ __forceinline__ void barrier_lds() {
   __builtin_amdgcn_s_barrier();
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
-
-// 0x80 in each byte that is a NaN code.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
 // Powers of two by which the value blocks of a workgroup may differ for f16 to hold their values exactly, and the
 // one that the largest block's codes are raised by: 448 * 2^7 is just below f16's largest, 2^-9 * 2^(7 - 12) its
@@ -963,7 +1036,7 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 // How a call is cut up, from its sizes alone (the lengths are on the device).
 struct Plan {
-  bool token;
+  int tiles;  // few rows: tiles of 16; 0 for more
   int64_t grid;
   int splits, rtiles;
   int64_t parts;  // partial rows of 128 + 2 floats
@@ -971,20 +1044,20 @@ struct Plan {
 
 Plan plan_of(int B, int H, int G, int T, int cap, int window, int sinks) {
   Plan p{};
-  p.token = T == 1 && G <= 16;
+  const int64_t R = static_cast<int64_t>(T) * G;
+  p.tiles = R <= 32 ? static_cast<int>((R + 15) / 16) : 0;
   // groups that a query can see: both ends of a window may lie inside one
   const int64_t keys = window ? std::min<int64_t>(cap, static_cast<int64_t>(window) + T - 1 + sinks) : cap;
-  if (p.token) {
+  if (p.tiles) {
     const int64_t groups = std::min<int64_t>((static_cast<int64_t>(cap) + kGroup - 1) / kGroup,
                                              (keys + kGroup - 1) / kGroup + 2);
     const int64_t each = (groups + kMinGroups - 1) / kMinGroups;
     const int64_t slots = std::min<int64_t>(B * each, (kTarget + H - 1) / H + B);
     p.grid = slots * H;
-    p.parts = p.grid * G;
+    p.parts = p.grid * R;
     p.splits = 1;
     return p;
   }
-  const int64_t R = static_cast<int64_t>(T) * G;
   p.rtiles = static_cast<int>((R + kRowsTile - 1) / kRowsTile);
   const int64_t wgs = static_cast<int64_t>(B) * H * p.rtiles;
   const int64_t tiles = (keys + kTile - 1) / kTile;
@@ -1058,9 +1131,9 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
          std::fabs(scale) * 1.44269504088896340736f, scale < 0.f, kTarget, p.splits, p.rtiles};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(p.grid)), t(256);
-  if (p.token) {
-    hipLaunchKernelGGL(token_kernel, g, t, 0, s, a);
-    hipLaunchKernelGGL(token_join_kernel, dim3(batch_size * q_heads), t, 0, s, a);
+  if (p.tiles) {
+    hipLaunchKernelGGL(p.tiles == 1 ? few_kernel<1> : few_kernel<2>, g, t, 0, s, a);
+    hipLaunchKernelGGL(few_join_kernel, dim3(batch_size * q_heads * rows), t, 0, s, a);
   } else {
     hipLaunchKernelGGL(rows_kernel, g, t, 0, s, a);
     if (p.splits > 1) hipLaunchKernelGGL(rows_join_kernel, dim3(batch_size * q_heads * rows), t, 0, s, a);
