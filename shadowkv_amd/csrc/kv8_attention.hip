@@ -152,7 +152,9 @@ __device__ __forceinline__ float sum_of_rows(float x) {
 constexpr int kGroup = 32;
 constexpr int kGroupShift = 5;
 constexpr int kMinGroups = 8;   // a chunk's groups of 32 keys, at least
-constexpr int kTarget = 1024;   // chunks to aim for: four workgroups to a CU
+// Chunks to aim for: four workgroups to a CU, twice that for up to 8 rows, whose partial results cost little (24
+// windows of 8256 keys, 4 rows: 80 -> 73 us; 16 rows, 4 sequences of 262143: 99 -> 111).
+constexpr int target_chunks(int64_t rows) { return rows <= 8 ? 2048 : 1024; }
 constexpr int kOutLd = kD + 4;
 
 struct Chunk {
@@ -255,12 +257,14 @@ __global__ void __launch_bounds__(256, kTiles == 1 ? 4 : 2) few_kernel(Args a) {
       kc[u] = ksh[blk];
       vc[u] = vsh[blk];
     }
+    // (values, whole rows of each line a load, with the streaming hint: 8 sequences of 122880 tokens 340 -> 317 us;
+    // keys, half of a line a load, gain nothing from it)
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int r = 0; r < 4; ++r)
-        vr[4 * u + r] = *reinterpret_cast<const u32x2*>(
-            vh + static_cast<int64_t>(min(j0 + 16 * u + 4 * grp + r, pmax)) * a.c_ss);
+        vr[4 * u + r] = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(
+            vh + static_cast<int64_t>(min(j0 + 16 * u + 4 * grp + r, pmax)) * a.c_ss));
   };
 
   for (int i = i0 + wave; i < i1; i += 4) {
@@ -1052,7 +1056,7 @@ Plan plan_of(int B, int H, int G, int T, int cap, int window, int sinks) {
     const int64_t groups = std::min<int64_t>((static_cast<int64_t>(cap) + kGroup - 1) / kGroup,
                                              (keys + kGroup - 1) / kGroup + 2);
     const int64_t each = (groups + kMinGroups - 1) / kMinGroups;
-    const int64_t slots = std::min<int64_t>(B * each, (kTarget + H - 1) / H + B);
+    const int64_t slots = std::min<int64_t>(B * each, (target_chunks(R) + H - 1) / H + B);
     p.grid = slots * H;
     p.parts = p.grid * R;
     p.splits = 1;
@@ -1128,7 +1132,8 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
   Args a{q, q_stride_b, q_stride_h, q_stride_t, k8, v8, c_stride_b, c_stride_h, c_stride_s, k_scale, v_scale,
          s_stride_b, s_stride_h, lengths, counts, out, ws_o, ws_o ? ws_o + p.parts * kD : nullptr, batch_size,
          kv_heads, q_heads / kv_heads, rows, cap, shift, window ? std::min(window, kNoWindow) : kNoWindow, sinks,
-         std::fabs(scale) * 1.44269504088896340736f, scale < 0.f, kTarget, p.splits, p.rtiles};
+         std::fabs(scale) * 1.44269504088896340736f, scale < 0.f,
+         target_chunks(static_cast<int64_t>(rows) * (q_heads / kv_heads)), p.splits, p.rtiles};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(p.grid)), t(256);
   if (p.tiles) {
