@@ -156,6 +156,12 @@ constexpr int kMinGroups = 8;   // a chunk's groups of 32 keys, at least
 // windows of 8256 keys, 4 rows: 80 -> 73 us; 16 rows, 4 sequences of 262143: 99 -> 111).
 constexpr int target_chunks(int64_t rows) { return rows <= 8 ? 2048 : 1024; }
 constexpr int kOutLd = kD + 4;
+// Groups that a sequence's rows can see (by the capacity and the window) up to which one workgroup of 16 waves (8 for
+// two tiles of rows) takes them all, in one launch, rather than chunks and a join: a window of 1024 keys with sinks,
+// its ends inside a group, or twice that where the sequences fill half of the chip (MI355X, us in a graph, 4 query heads
+// on each of 8 kv heads, chunks / whole: 1 sequence of 512 keys 10.0 / 7.6, 1024 9.9 / 10.1 and a launch less from the
+// host, 2048 10.0 / 15.8; 24 sequences of 1024 16.4 / 11.8, 2048 26.1 / 20.2).
+constexpr int whole_groups(int tiles, int64_t rows_of_kv) { return (rows_of_kv >= 128 ? 72 : 36) / tiles; }
 
 struct Chunk {
   int b, index, groups;  // sequence, which of its chunks, groups of a chunk
@@ -198,20 +204,24 @@ __device__ __forceinline__ bool find_chunk(const Args& a, int i, int lane, Chunk
 // 0x80 in each byte that is a NaN code.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-template <int kTiles>  // of 16 rows
-__global__ void __launch_bounds__(256, kTiles == 1 ? 4 : 2) few_kernel(Args a) {
-  __shared__ float o_lds[4][16][kOutLd];
-  __shared__ float m_lds[4][16], l_lds[4][16];
+// kTiles: of 16 rows. kWhole: a workgroup of more waves takes all that a sequence's rows see, and writes its result.
+constexpr int few_threads(int tiles, bool whole) { return 64 * (whole ? 16 / tiles : 4); }
+
+template <int kTiles, bool kWhole>
+__global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 : 2) few_kernel(Args a) {
+  constexpr int kWaves = few_threads(kTiles, kWhole) / 64;
+  __shared__ float o_lds[kWaves][16][kOutLd];
+  __shared__ float m_lds[kWaves][16], l_lds[kWaves][16];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int slot = blockIdx.x / a.H, h = blockIdx.x - slot * a.H;
-  Chunk c;
-  if (!find_chunk(a, slot, lane, c)) return;  // workgroup-uniform
+  Chunk c{slot, 0, 1 << 30};
+  if (!kWhole && !find_chunk(a, slot, lane, c)) return;  // workgroup-uniform
   const int b = c.b, G = a.G, R = G * a.T;
   const int len = length_of(a, b), n = count_of(a, b);
   const int pmin = len - n, pmax = len - 1;
   const Groups seen = few_groups(a, b);
-  const int i0 = c.index * c.groups, i1 = min(i0 + c.groups, seen.total);
+  const int i0 = kWhole ? 0 : c.index * c.groups, i1 = kWhole ? seen.total : min(i0 + c.groups, seen.total);
   const int li = lane & 15, grp = lane >> 4;
 
   // Q as the B operand: lane (li, grp) holds row li of a tile, in step s dims 64 (s / 2) + 16 grp + 8 (s % 2) and on.
@@ -267,7 +277,7 @@ __global__ void __launch_bounds__(256, kTiles == 1 ? 4 : 2) few_kernel(Args a) {
             vh + static_cast<int64_t>(min(j0 + 16 * u + 4 * grp + r, pmax)) * a.c_ss));
   };
 
-  for (int i = i0 + wave; i < i1; i += 4) {
+  for (int i = i0 + wave; i < i1; i += kWaves) {
     load(i);
     const int j0 = seen.at(i) * kGroup;
     f32x4 s[kTiles][2];
@@ -408,20 +418,28 @@ __global__ void __launch_bounds__(256, kTiles == 1 ? 4 : 2) few_kernel(Args a) {
               f32x4{o[y][e][r], o[y][e + 1][r], o[y][e + 2][r], o[y][e + 3][r]};
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * 32; i += 256) {
+    for (int i = threadIdx.x; i < rows * 32; i += 64 * kWaves) {
       const int g = i >> 5, d = 4 * (i & 31), row = 16 * y + g;
       const bool query = row / G < n;  // (padding: as if it had seen nothing)
       float top = m_lds[0][g];
 #pragma unroll
-      for (int w = 1; w < 4; ++w) top = fmaxf(top, m_lds[w][g]);
+      for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][g]);
       const float ref = top == -INFINITY ? 0.f : top;
       f32x4 sum = {0.f, 0.f, 0.f, 0.f};
       float lsum = 0.f;
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
+      for (int w = 0; w < kWaves; ++w) {
         const float f = __builtin_amdgcn_exp2f(m_lds[w][g] - ref);
         lsum += f * l_lds[w][g];
         sum += f * *reinterpret_cast<const f32x4*>(&o_lds[w][g][d]);
+      }
+      if constexpr (kWhole) {
+        const float inv = query && lsum != 0.f ? 1.f / lsum : 0.f;  // (nothing seen: zeros)
+        const u32x2 out = {skv::f2bf2(sum[0] * inv, sum[1] * inv), skv::f2bf2(sum[2] * inv, sum[3] * inv)};
+        const int t = row / G;
+        *reinterpret_cast<u32x2*>(a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H * G + h * G + row - t * G) * kD + d) =
+            query ? out : u32x2{0u, 0u};
+        continue;
       }
       *reinterpret_cast<f32x4*>(a.ws_o + (row0 + row) * kD + d) = query ? sum : f32x4{0.f, 0.f, 0.f, 0.f};
       if (d == 0) {
@@ -1040,7 +1058,8 @@ bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p
 
 // How a call is cut up, from its sizes alone (the lengths are on the device).
 struct Plan {
-  int tiles;  // few rows: tiles of 16; 0 for more
+  int tiles;   // few rows: tiles of 16; 0 for more
+  bool whole;  // few rows: one workgroup a (sequence, kv head)
   int64_t grid;
   int splits, rtiles;
   int64_t parts;  // partial rows of 128 + 2 floats
@@ -1055,6 +1074,11 @@ Plan plan_of(int B, int H, int G, int T, int cap, int window, int sinks) {
   if (p.tiles) {
     const int64_t groups = std::min<int64_t>((static_cast<int64_t>(cap) + kGroup - 1) / kGroup,
                                              (keys + kGroup - 1) / kGroup + 2);
+    p.whole = groups <= whole_groups(p.tiles, static_cast<int64_t>(B) * H);
+    if (p.whole) {
+      p.grid = static_cast<int64_t>(B) * H;
+      return p;
+    }
     const int64_t each = (groups + kMinGroups - 1) / kMinGroups;
     const int64_t slots = std::min<int64_t>(B * each, (target_chunks(R) + H - 1) / H + B);
     p.grid = slots * H;
@@ -1136,8 +1160,12 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
          target_chunks(static_cast<int64_t>(rows) * (q_heads / kv_heads)), p.splits, p.rtiles};
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(p.grid)), t(256);
-  if (p.tiles) {
-    hipLaunchKernelGGL(p.tiles == 1 ? few_kernel<1> : few_kernel<2>, g, t, 0, s, a);
+  if (p.whole) {
+    if (p.tiles == 1) hipLaunchKernelGGL((few_kernel<1, true>), g, dim3(few_threads(1, true)), 0, s, a);
+    else hipLaunchKernelGGL((few_kernel<2, true>), g, dim3(few_threads(2, true)), 0, s, a);
+  } else if (p.tiles) {
+    if (p.tiles == 1) hipLaunchKernelGGL((few_kernel<1, false>), g, t, 0, s, a);
+    else hipLaunchKernelGGL((few_kernel<2, false>), g, t, 0, s, a);
     hipLaunchKernelGGL(few_join_kernel, dim3(batch_size * q_heads * rows), t, 0, s, a);
   } else {
     hipLaunchKernelGGL(rows_kernel, g, t, 0, s, a);

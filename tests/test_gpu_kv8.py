@@ -271,13 +271,15 @@ def _queries(B, Hq, T, gen, gpu, size=1.0):
 
 @pytest.mark.parametrize("G", [1, 4, 7, 16])
 @pytest.mark.parametrize("block", [16, 32, 64, 128])
-def test_attn_one_token(gpu, G, block):
-    """Lengths from none to the whole capacity, around the groups of 32 keys and the chunks of 256; everything
-    behind a sequence's end is garbage (NaN codes and scales among it)."""
-    _say(f"kv8_attn one token G={G} block={block}")
+@pytest.mark.parametrize("cap", [700, 2500])
+def test_attn_one_token(gpu, G, block, cap):
+    """Lengths from none to the whole capacity, around the groups of 32 keys and the chunks of 256 (a capacity that one
+    workgroup takes, and one that is cut); everything behind a sequence's end is garbage (NaN codes and scales
+    among it)."""
+    _say(f"kv8_attn one token G={G} block={block} cap={cap}")
     g = torch.Generator().manual_seed(G * block)
-    H, cap = 2, 700
-    lengths = [0, 1, 15, 16, 31, 32, 33, 64, 129, 255, 256, 257, 300, 513, 699, 700, 900, -3]
+    H = 2
+    lengths = [0, 1, 15, 16, 31, 32, 33, 64, 129, 255, 256, 257, 300, 513, 699, 700, cap + 200, -3]
     caches = _filled(len(lengths), H, cap, block, g, gpu)
     for b, n in enumerate(lengths):
         n = max(n, 0)
@@ -290,12 +292,13 @@ def test_attn_one_token(gpu, G, block):
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (31, 4), (64, 0), (100, 33), (300, 64), (5000, 3), (200, 5000)])
-def test_attn_one_token_window(gpu, window, sinks):
+@pytest.mark.parametrize("cap", [640, 2500])
+def test_attn_one_token_window(gpu, window, sinks, cap):
     """Windows and sinks that begin and end inside a group, meet, and cover everything; hidden keys and values are
     NaN where a whole group or a part of one is hidden."""
-    _say(f"kv8_attn one token window={window} sinks={sinks}")
+    _say(f"kv8_attn one token window={window} sinks={sinks} cap={cap}")
     g = torch.Generator().manual_seed(window + sinks)
-    H, G, block, cap = 2, 4, 32, 640
+    H, G, block = 2, 4, 32
     lengths = [1, 30, 65, 99, 101, 333, 400, 401, 431, 639, 640]
     caches = _filled(len(lengths), H, cap, block, g, gpu)
     for b, n in enumerate(lengths):
@@ -310,12 +313,12 @@ def test_attn_one_token_window(gpu, window, sinks):
 @pytest.mark.parametrize("H,G,T", [(2, 4, 2), (1, 1, 33), (3, 7, 19), (2, 17, 1), (1, 40, 1), (2, 16, 9), (8, 4, 70),
                                    (1, 4, 300)])
 @pytest.mark.parametrize("block", [16, 128])
-def test_attn_many(gpu, H, G, T, block):
+@pytest.mark.parametrize("cap", [450, 2500])
+def test_attn_many(gpu, H, G, T, block, cap):
     """Several tokens, or more than 16 heads a kv head: rows around the tiles of 32 and 128, lengths around the
     tiles of 64 and shorter than the new tokens, ragged counts; garbage behind the ends."""
-    _say(f"kv8_attn many H={H} G={G} T={T} block={block}")
+    _say(f"kv8_attn many H={H} G={G} T={T} block={block} cap={cap}")
     g = torch.Generator().manual_seed(H * G + T)
-    cap = 450
     lengths = [T, T + 1, 0, 64, 65, 191, 450, max(1, T // 2), 3000]
     counts = [T, max(1, T - 1), 1, T, T // 2, T, 0, T, T + 5]
     caches = _filled(len(lengths), H, cap, block, g, gpu, "bsh" if T == 19 else "bhs")
@@ -330,26 +333,26 @@ def test_attn_many(gpu, H, G, T, block):
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 2), (63, 1), (64, 64), (100, 33), (130, 0), (4000, 7), (90, 4000)])
-@pytest.mark.parametrize("T", [5, 150])
-def test_attn_many_window(gpu, window, sinks, T):
+@pytest.mark.parametrize("T,cap", [(5, 700), (5, 2500), (150, 700)])
+def test_attn_many_window(gpu, window, sinks, T, cap):
     """Windows with sinks over several tokens, each with its own end."""
-    _say(f"kv8_attn many window={window} sinks={sinks} T={T}")
+    _say(f"kv8_attn many window={window} sinks={sinks} T={T} cap={cap}")
     g = torch.Generator().manual_seed(window + sinks + T)
     lengths, counts = [T, 333, 700, 640, 65, 700], [T, T, T, T // 2, 1, max(1, T - 3)]
-    caches = _filled(len(lengths), 2, 700, 64, g, gpu)
+    caches = _filled(len(lengths), 2, cap, 64, g, gpu)
     q = _queries(len(lengths), 8, T, g, gpu, 1.5)
     _check_attn(q, caches, lengths, counts, 64, window, sinks)
 
 
-@pytest.mark.parametrize("T", [1, 2, 70])
-def test_attn_nan_where_seen_and_hidden(gpu, T):
+@pytest.mark.parametrize("T,cap", [(1, 320), (2, 320), (2, 2500), (6, 2500), (70, 320)])
+def test_attn_nan_where_seen_and_hidden(gpu, T, cap):
     """A NaN among the keys makes the rows that see it NaN, one among the values the dims of the rows that see it,
     and neither reaches a row that does not (a later key, or one behind the window)."""
-    _say(f"kv8_attn NaN T={T}")
+    _say(f"kv8_attn NaN T={T} cap={cap}")
     g = torch.Generator().manual_seed(T)
     lengths = [300, 300, 299]
     for window, sinks in ((None, 0), (40, 10)):
-        caches = _filled(3, 2, 320, 32, g, gpu)
+        caches = _filled(3, 2, cap, 32, g, gpu)
         v8, k8 = caches[1].view(torch.uint8), caches[0].view(torch.uint8)
         v8[0, 0, 299, 5] = v8[0, 1, 270, 9] = v8[0, 1, 3, 127] = 0x7f
         v8[1, 0, 250, 64:70] = 0xff
@@ -364,12 +367,12 @@ def test_attn_nan_where_seen_and_hidden(gpu, T):
         assert torch.equal(got[1, :, 4:].isnan().any(-1), see.unsqueeze(1).expand(T, 4))
 
 
-@pytest.mark.parametrize("T", [3, 45])
-def test_attn_padding_beside_nan(gpu, T):
+@pytest.mark.parametrize("T,cap", [(3, 128), (3, 2500), (45, 128)])
+def test_attn_padding_beside_nan(gpu, T, cap):
     """Padding rows are zeros where the sequence's own rows are NaN, and where their queries are NaN or infinite."""
-    _say(f"kv8_attn padding beside NaN T={T}")
+    _say(f"kv8_attn padding beside NaN T={T} cap={cap}")
     g = torch.Generator().manual_seed(T)
-    caches = _filled(2, 2, 128, 32, g, gpu)
+    caches = _filled(2, 2, cap, 32, g, gpu)
     caches[1].view(torch.uint8)[:, :, 60] = 0x7f
     q = _queries(2, 8, T, g, gpu)
     q[:, :, T - 1] = math.nan
