@@ -626,13 +626,11 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   };
   u32x4 kheld[2];
   uint32_t vheld[8];
-  auto fetch_keys = [&](const Lane& x, int tile) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t src = tile_rows(kh, tile);
+  auto fetch_keys = [&](const Lane& x, __amdgpu_buffer_rsrc_t src) __attribute__((always_inline)) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) kheld[c] = __builtin_amdgcn_raw_buffer_load_b128(src, x.kmine, 16 * c, 0);
   };
-  auto fetch_values = [&](const Lane& x, int tile) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t src = tile_rows(vh, tile);
+  auto fetch_values = [&](const Lane& x, __amdgpu_buffer_rsrc_t src) __attribute__((always_inline)) {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       vheld[e] = __builtin_amdgcn_raw_buffer_load_b32(src, x.vmine, ((e & 3) + 8 * (e >> 2)) * stride, 0);
@@ -764,18 +762,27 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   // one barrier a tile, and vector work beside every matrix instruction. The order is written down slice by slice (a
   // scheduler of its own would read all operands first, and spill).
   auto walk_whole = [&](int from, int to) __attribute__((always_inline)) {
-    if (from >= to) return;  // workgroup-uniform
-    __syncthreads();         // every wave is past the tiles before these
+    __syncthreads();  // every wave is past the tiles before these
     const Lane g = own_lane();
     int kbase = k_at(g.li, g.half);
-    const int end = to - 1;
-    auto tile_at = [&](int i) __attribute__((always_inline)) { return seen.at(min(i, end)); };
-    // Scales of a tile's groups of 16 keys, a tile ahead, in a lane each: the keys' in lanes 0 to 3, the values' in 4 to 7.
-    float held_scales[3];
-    auto fetch_scales = [&](int tile) __attribute__((always_inline)) {
-      return (g.li & 4 ? vsh : ksh)[block_of(tile, g.li & 3)];
+    const int end = to - 1;  // (tiles one behind the other, none cut off by the sequence's end)
+    const uint64_t tile_bytes = static_cast<uint64_t>(kTile) * stride;
+    auto whole_rows = [&](const uint8_t* base, int tile) __attribute__((always_inline)) {
+      return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + min(tile, end) * tile_bytes), 0,
+                                               (kTile - 1) * stride + kD, kDw3);
     };
-    auto lane_scale = [&](float held, int which) __attribute__((always_inline)) {
+    // The factors of a tile's groups of 16 keys in a lane each: the keys' in lanes 0 to 3, the values' in 4 to 7. Of tiles
+    // i and i + 1, and the scales of i + 2.
+    float factors[2], scales;
+    const float* own_scales = g.li & 4 ? vsh : ksh;
+    auto fetch_scales = [&](int tile) __attribute__((always_inline)) {
+      return own_scales[(min(tile, end) * kTile + 16 * (g.li & 3)) >> a.block_shift];
+    };
+    auto factors_of = [&](float scale) __attribute__((always_inline)) {
+      const float k = key_factor(scale, a.scale_log2e), v = value_factor(scale);
+      return g.li & 4 ? v : k;
+    };
+    auto lane_factor = [&](float held, int which) __attribute__((always_inline)) {
       return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), which));
     };
     // One tile: its scores in s, the next one's into sn (past the last, the last one's again). Keys i are in kt[par],
@@ -795,8 +802,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       for (int j = 0; j < 3; ++j) operand(j);
       float kf[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) kf[q] = key_factor(lane_scale(held_scales[0], q), a.scale_log2e);
-      const float factor = value_factor(lane_scale(held_scales[1], 4 + wave));
+      for (int q = 0; q < 4; ++q) kf[q] = lane_factor(factors[0], q);
+      const float factor = lane_factor(factors[1], 4 + wave);
       float mx = -INFINITY, ref = 0.f;
       auto largest_of = [&](int q) __attribute__((always_inline)) {
         mx = fmaxf(mx, max8(s[q >> 1], 8 * (q & 1)) * kf[q]);
@@ -842,32 +849,33 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
 #pragma unroll
             for (int z = 0; z < 2; ++z) vt[par ^ 1][v_at(wave, g.half, 4 * g.li + 2 * y + z)] = x[z];
         } else if (j == 28) {
-          fetch_keys(g, tile_at(i + 3));
+          fetch_keys(g, whole_rows(kh, i + 3));
         } else if (j == 29) {
-          fetch_values(g, tile_at(i + 2));
+          fetch_values(g, whole_rows(vh, i + 2));
         } else if (j == 30) {
-          held_scales[0] = held_scales[1];
-          held_scales[1] = held_scales[2];
-          held_scales[2] = fetch_scales(tile_at(i + 3));
+          factors[0] = factors[1];
+          factors[1] = factors_of(scales);
+          scales = fetch_scales(i + 3);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
     };
-    fetch_keys(g, tile_at(from));
-    fetch_values(g, tile_at(from));
+    fetch_keys(g, whole_rows(kh, from));
+    fetch_values(g, whole_rows(vh, from));
     place_keys(g, 0);
-    place_f16(g, tile_at(from), 0);
+    place_f16(g, from, 0);
     __builtin_amdgcn_sched_barrier(0);
-    fetch_keys(g, tile_at(from + 1));
+    fetch_keys(g, whole_rows(kh, from + 1));
     place_keys(g, 1);
     __builtin_amdgcn_sched_barrier(0);
-    fetch_keys(g, tile_at(from + 2));
-    fetch_values(g, tile_at(from + 1));
+    fetch_keys(g, whole_rows(kh, from + 2));
+    fetch_values(g, whole_rows(vh, from + 1));
     __syncthreads();
     f32x16 sa[2], sb[2];
     scores(g, 0, sa);
-#pragma unroll
-    for (int t = 0; t < 3; ++t) held_scales[t] = fetch_scales(tile_at(from + t));
+    factors[0] = factors_of(fetch_scales(from));
+    factors[1] = factors_of(fetch_scales(from + 1));
+    scales = fetch_scales(from + 2);
     for (int i = from;;) {
       step(std::integral_constant<int, 0>{}, i, sa, sb);
       if (++i > end) break;
@@ -910,8 +918,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     const Row mine = row_of(g.li);
     const int p = mine.query ? p0 + mine.t : pmax;
     __syncthreads();  // every wave is past the tiles before these
-    fetch_keys(g, seen.at(from));
-    fetch_values(g, seen.at(from));
+    fetch_keys(g, tile_rows(kh, seen.at(from)));
+    fetch_values(g, tile_rows(vh, seen.at(from)));
     for (int i = from; i < to; ++i) {
       const int buf = (i - from) & 1, tile = seen.at(i);
       place_keys(g, buf);
@@ -919,8 +927,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       else place_any(g, buf);
       __syncthreads();  // (and every wave is past the tile before last, whose place the next one takes)
       if (i + 1 < to) {
-        fetch_keys(g, seen.at(i + 1));
-        fetch_values(g, seen.at(i + 1));
+        fetch_keys(g, tile_rows(kh, seen.at(i + 1)));
+        fetch_values(g, tile_rows(vh, seen.at(i + 1)));
       }
       f32x16 s[2];
       float kf[4];
@@ -979,7 +987,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     }
   };
 
-  // Of tiles i0 to i1 - 1 those that every row sees whole: j0 to j1 - 1.
+  // Of the tiles that are seen, i0 to i1 - 1, those that every row sees whole and that lie one behind the other: j0 to
+  // j1 - 1.
   const int low = a.window < kNoWindow ? max(0, pmax - a.window + kTile) >> kTileShift : 0;
   const int j0 = min(max(seen.index(low), i0), i1), j1 = min(max(seen.index((pmin + 1) >> kTileShift), j0), i1);
   clear();
@@ -988,7 +997,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     bool exact = fits;
     if (fits) {
       walk(std::true_type{}, i0, j0);
-      walk_whole(j0, j1);
+      if (j0 < j1) walk_whole(seen.at(j0), seen.at(j0) + j1 - j0);
       walk(std::true_type{}, j1, i1);
       back = __builtin_ldexpf(1.f, vtop - 127 - kRaise);
       // NaN anywhere: a value may have reached rows that do not see it.
