@@ -145,7 +145,7 @@ struct ReadArgs {
   const int64_t* ids;  // [B, H, chunks] or null
   uint16_t* out;       // [B, H, rows, 128]
   int64_t start;
-  int H, cap, block, chunk, rows, groups;
+  int H, cap, block, chunk, chunks, rows, groups;  // chunks: that begin inside the cache
 };
 
 constexpr int kReadRows = 128;  // rows of a workgroup, 8 lanes of 16 elements each, 4 in flight a thread
@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
     bool ok = true;
     if (a.ids) {
       const int64_t id = a.ids[static_cast<int64_t>(bh) * (a.rows / a.chunk) + r / a.chunk];
-      ok = id >= 0 && id < (a.cap + a.chunk - 1) / a.chunk;
+      ok = id >= 0 && id < a.chunks;
       at = (ok ? id : 0) * a.chunk + r % a.chunk;
     }
     ok = ok && at < a.cap;
@@ -193,6 +193,9 @@ __global__ void __launch_bounds__(kThreads) read_kernel(ReadArgs a) {
   }
 }
 
+constexpr int64_t kMaxThreads = int64_t{1} << 32;  // of a launch
+constexpr int kMaxTokens = 1 << 30;
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 bool block_ok(int block) { return block == 16 || block == 32 || block == 64 || block == 128; }
@@ -210,7 +213,7 @@ extern "C" int skv_kv8_write(const uint16_t* k, int64_t k_stride_b, int64_t k_st
     skv_set_error("%s: null pointer", what);
     return SKV_EINVAL;
   }
-  if (batch_size < 1 || heads < 1 || rows < 1 || cap < 1) {
+  if (batch_size < 1 || heads < 1 || rows < 1 || rows > kMaxTokens || cap < 1 || cap > kMaxTokens) {
     skv_set_error("%s: batch=%d heads=%d rows=%d cap=%d", what, batch_size, heads, rows, cap);
     return SKV_EINVAL;
   }
@@ -226,7 +229,7 @@ extern "C" int skv_kv8_write(const uint16_t* k, int64_t k_stride_b, int64_t k_st
   }
   const int64_t blocks = (static_cast<int64_t>(rows) + block - 2) / block + 1;
   const int64_t grid = blocks * heads * batch_size * 2;
-  if (grid > (int64_t{1} << 30)) {
+  if (grid * kThreads >= kMaxThreads) {
     skv_set_error("%s: batch=%d heads=%d rows=%d", what, batch_size, heads, rows);
     return SKV_EUNSUPPORTED;
   }
@@ -253,8 +256,8 @@ extern "C" int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_
     skv_set_error("%s: null pointer", what);
     return SKV_EINVAL;
   }
-  if (batch_size < 1 || heads < 1 || rows < 1 || cap < 1 || start < 0 ||
-      (chunk_ids ? chunk_size < 1 || rows % chunk_size || start : start + rows > cap)) {
+  if (batch_size < 1 || heads < 1 || rows < 1 || rows > kMaxTokens || cap < 1 || cap > kMaxTokens || start < 0 ||
+      (chunk_ids ? chunk_size < 1 || rows % chunk_size || start : start > cap - rows)) {
     skv_set_error("%s: batch=%d heads=%d start=%lld rows=%d chunk=%d cap=%d", what, batch_size, heads,
                   (long long)start, rows, chunk_size, cap);
     return SKV_EINVAL;
@@ -270,12 +273,13 @@ extern "C" int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_
   }
   const int64_t groups = (static_cast<int64_t>(rows) + kReadRows - 1) / kReadRows;
   const int64_t grid = groups * heads * batch_size;
-  if (grid > (int64_t{1} << 30)) {
+  if (grid * kThreads >= kMaxThreads) {
     skv_set_error("%s: batch=%d heads=%d rows=%d", what, batch_size, heads, rows);
     return SKV_EUNSUPPORTED;
   }
+  const int chunk = chunk_ids ? chunk_size : 1;
   ReadArgs a{codes, scale, c_stride_b, c_stride_h, c_stride_s, s_stride_b, s_stride_h, chunk_ids, out, start, heads,
-             cap, block, chunk_ids ? chunk_size : 1, rows, static_cast<int>(groups)};
+             cap, block, chunk, static_cast<int>((static_cast<int64_t>(cap) + chunk - 1) / chunk), rows, static_cast<int>(groups)};
   hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
                      a);
   return skv_check_launch(what);

@@ -298,22 +298,34 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
 #pragma unroll
         for (int r = 0; r < 4; ++r) s[y][u][r] *= f;
     }
+    float vf[kTiles][2];  // the value blocks' factors
+#pragma unroll
+    for (int y = 0; y < kTiles; ++y)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) vf[y][u] = vc[u];
     // wave-uniform: a group at an end of what a row sees
     if (j0 + kGroup > pmin + 1 || (j0 <= pmax - a.window && j0 + kGroup > a.sinks)) {
       uint32_t odd = 0;
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
+      for (int u = 0; u < 2; ++u) {
+        bool some[kTiles] = {};
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const int j = j0 + 16 * u + 4 * grp + r;
 #pragma unroll
-          for (int y = 0; y < kTiles; ++y)
-            if (!sees(p[y], j, a.window, a.sinks)) s[y][u][r] = -INFINITY;
+          for (int y = 0; y < kTiles; ++y) {
+            const bool yes = sees(p[y], j, a.window, a.sinks);
+            s[y][u][r] = yes ? s[y][u][r] : -INFINITY;
+            some[y] |= yes;
+          }
           // a value that no row sees may be anything: zero codes
           u32x2& w = vr[4 * u + r];
           if (!(j <= pmax && (j > pmin - a.window || j < a.sinks))) w = u32x2{0u, 0u};
           odd |= nan_bytes(w[0]) | nan_bytes(w[1]);
         }
+#pragma unroll
+        for (int y = 0; y < kTiles; ++y) vf[y][u] = some[y] ? vf[y][u] : 0.f;  // (so may its scale)
+      }
       if (n > 1 && __any(odd != 0)) {  // wave-uniform
         // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
         // would: a hidden key's zero times NaN): how many such keys a row sees is a product of its own.
@@ -374,7 +386,7 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
           const float p0 = __builtin_amdgcn_exp2f(s[y][u][r] - ref), p1 = __builtin_amdgcn_exp2f(s[y][u][r + 1] - ref);
           l[y] += p0 + p1;
           uint32_t first, second;
-          two_parts(p0 * vc[u], p1 * vc[u], first, second);
+          two_parts(p0 * vf[y][u], p1 * vf[y][u], first, second);
           part[y][0][2 * u + r / 2] = first;
           part[y][1][2 * u + r / 2] = second;
         }
@@ -384,8 +396,8 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
       uint32_t w[8];
 #pragma unroll
       for (int t = 0; t < 8; ++t) w[t] = vr[t][half];
-      u32x4 vf[4];
-      transpose_bf16(w, vf);
+      u32x4 vt[4];
+      transpose_bf16(w, vt);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -393,7 +405,7 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
 #pragma unroll
           for (int y = 0; y < kTiles; ++y)
             o[y][4 * half + e] =
-                __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vf[e]),
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vt[e]),
                                                         __builtin_bit_cast(bf16x8, part[y][x]), o[y][4 * half + e], 0, 0, 0);
     }
   }
@@ -513,9 +525,7 @@ constexpr int kRowsTile = 4 * kRowsWave;
 
 // 16-byte chunk c (8 dims) of key row r of a tile in LDS, and chunk (group of 16 keys, half of its order, dim).
 __device__ __forceinline__ int k_at(int r, int c) { return r * 16 + (c ^ (r & 15)); }
-__device__ __forceinline__ int v_at(int gk, int half, int d) { return gk * 256 + half * 128 + (d ^ ((d >> 4) & 3)); }
-
-__device__ __forceinline__ u32x4 load4(const uint8_t* p) { return *reinterpret_cast<const u32x4*>(p); }
+__device__ __forceinline__ int v_at(int gk, int half, int d) { return gk * 256 + half * 128 + (d ^ ((d >> 3) & 7)); }
 
 // The largest of eight, four instructions (fmaxf would first quiet each operand that comes from a matrix instruction).
 // Not right behind the one that makes them: the compiler does not see what this waits for.
@@ -696,15 +706,12 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
     return fmaxf(__uint_as_float(w[0]), __uint_as_float(w[1]));
   };
-  auto largest = [&](const f32x16 (&s)[2], const float (&kf)[4]) __attribute__((always_inline)) {
+  auto largest = [&](const f32x16 (&s)[2]) __attribute__((always_inline)) {
     float mx = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      float y = s[q >> 1][8 * (q & 1)];
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-      for (int r = 1; r < 8; ++r) y = fmaxf(y, s[q >> 1][8 * (q & 1) + r]);
-      mx = fmaxf(mx, y * kf[q]);
-    }
+      for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[u][r]);
     return largest_half(mx);
   };
   // The reference moves only when a score passes it by 2^kSlack: the ratio of the sums does not depend on it.
@@ -757,10 +764,10 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     put_values(x, o4, buf);
   };
 
-  // Tiles that every row sees whole, values and probabilities in f16, one product. Tile i's probabilities and their product are taken
-  // while tile i + 1's scores are, tile i + 2's keys and i + 1's values go to LDS and the next ones are on their way:
-  // one barrier a tile, and vector work beside every matrix instruction. The order is written down slice by slice (a
-  // scheduler of its own would read all operands first, and spill).
+  // Tiles that every row sees whole, values and probabilities in f16, one product. Tile i's probabilities and their
+  // product are taken while tile i + 1's scores are, tile i + 2's keys and i + 1's values go to LDS and the next ones
+  // are on their way: one barrier a tile, and vector work beside every matrix instruction. The order is written down
+  // slice by slice (a scheduler of its own would read all operands first, and spill).
   auto walk_whole = [&](int from, int to) __attribute__((always_inline)) {
     __syncthreads();  // every wave is past the tiles before these
     const Lane g = own_lane();
@@ -935,9 +942,13 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       scores(g, buf, s);
       key_scales(tile, kf);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) kf[q] = key_factor(kf[q], a.scale_log2e);
-      hide(g, p, tile, s);
-      const float ref = refer(largest(s, kf));
+      for (int q = 0; q < 4; ++q) {
+        const float f = key_factor(kf[q], a.scale_log2e);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[q >> 1][8 * (q & 1) + r] *= f;
+      }
+      hide(g, p, tile, s);  // (behind the factors: a hidden block's scale may be anything)
+      const float ref = refer(largest(s));
       if constexpr (!kF16) {
         for (int q = 0; q < 4; ++q) {
           // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
@@ -956,8 +967,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
         u32x4 part[2];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const float x0 = __builtin_amdgcn_exp2f(fmaf(s[gk >> 1][8 * (gk & 1) + 2 * e], kf[gk], -ref));
-          const float x1 = __builtin_amdgcn_exp2f(fmaf(s[gk >> 1][8 * (gk & 1) + 2 * e + 1], kf[gk], -ref));
+          const float x0 = __builtin_amdgcn_exp2f(s[gk >> 1][8 * (gk & 1) + 2 * e] - ref);
+          const float x1 = __builtin_amdgcn_exp2f(s[gk >> 1][8 * (gk & 1) + 2 * e + 1] - ref);
           if constexpr (kF16) {
             const f16x2 x = __builtin_convertvector(f32x2{x0, x1}, f16x2);
             l = __builtin_amdgcn_fdot2(x, f16x2{1, 1}, l, false);  // (the sum of what the product takes)
@@ -965,7 +976,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
           } else {
             l += x0 + x1;
             uint32_t first, second;
-            two_parts(x0 * vsc, x1 * vsc, first, second);
+            // (a hidden block's scale may be anything)
+            two_parts(x0 == 0.f ? 0.f : x0 * vsc, x1 == 0.f ? 0.f : x1 * vsc, first, second);
             part[0][e] = first;
             part[1][e] = second;
           }
@@ -1063,6 +1075,8 @@ __global__ void __launch_bounds__(256) rows_join_kernel(Args a) {
              a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H * a.G + h * a.G + g) * kD, acc_lds);
 }
 
+constexpr int64_t kMaxThreads = int64_t{1} << 32;  // of a launch
+
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 // How a call is cut up, from its sizes alone (the lengths are on the device).
@@ -1155,7 +1169,9 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
                   (long long)need);
     return SKV_EINVAL;
   }
-  if (p.grid > (int64_t{1} << 30)) {
+  const int threads = p.whole ? few_threads(p.tiles, true) : 256;
+  const int64_t join = p.parts ? static_cast<int64_t>(batch_size) * q_heads * rows : 0;  // workgroups of it
+  if (p.grid * threads >= kMaxThreads || join * 256 >= kMaxThreads) {
     skv_set_error("%s: batch=%d q_heads=%d rows=%d", what, batch_size, q_heads, rows);
     return SKV_EUNSUPPORTED;
   }
@@ -1170,15 +1186,15 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
   const hipStream_t s = static_cast<hipStream_t>(stream);
   const dim3 g(static_cast<unsigned>(p.grid)), t(256);
   if (p.whole) {
-    if (p.tiles == 1) hipLaunchKernelGGL((few_kernel<1, true>), g, dim3(few_threads(1, true)), 0, s, a);
-    else hipLaunchKernelGGL((few_kernel<2, true>), g, dim3(few_threads(2, true)), 0, s, a);
+    if (p.tiles == 1) hipLaunchKernelGGL((few_kernel<1, true>), g, dim3(threads), 0, s, a);
+    else hipLaunchKernelGGL((few_kernel<2, true>), g, dim3(threads), 0, s, a);
   } else if (p.tiles) {
     if (p.tiles == 1) hipLaunchKernelGGL((few_kernel<1, false>), g, t, 0, s, a);
     else hipLaunchKernelGGL((few_kernel<2, false>), g, t, 0, s, a);
-    hipLaunchKernelGGL(few_join_kernel, dim3(batch_size * q_heads * rows), t, 0, s, a);
+    hipLaunchKernelGGL(few_join_kernel, dim3(static_cast<unsigned>(join)), t, 0, s, a);
   } else {
     hipLaunchKernelGGL(rows_kernel, g, t, 0, s, a);
-    if (p.splits > 1) hipLaunchKernelGGL(rows_join_kernel, dim3(batch_size * q_heads * rows), t, 0, s, a);
+    if (p.splits > 1) hipLaunchKernelGGL(rows_join_kernel, dim3(static_cast<unsigned>(join)), t, 0, s, a);
   }
   return skv_check_launch(what);
 }

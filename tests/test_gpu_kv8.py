@@ -404,6 +404,82 @@ def test_attn_scores_of_every_size(gpu, T):
         _check_attn(q, caches, [L], None, 16, scale=0.01)
 
 
+@pytest.mark.parametrize("T,cap", [(1, 320), (7, 320), (1, 2500), (7, 2500), (70, 320), (70, 2500)])
+def test_attn_scales_that_are_hidden(gpu, T, cap):
+    """Scales of blocks that a query does not see, behind its window or past the sequence's end, may be anything, and
+    so may the codes there; a query that does see a block of NaN scales is NaN."""
+    _say(f"kv8_attn hidden scales T={T} cap={cap}")
+    g = torch.Generator().manual_seed(T + cap)
+    odd = [math.nan, math.inf, -math.inf, -1.0]
+    lengths, window, sinks = [300, 231], 30, 5
+    for which in range(4):
+        caches = _filled(2, 2, cap, 16, g, gpu)
+        want = [c.clone() for c in caches]
+        for b, L in enumerate(lengths):
+            first = max(0, L - T - window + 1) // 16  # (the sinks' block is seen)
+            for c, ones in zip(caches, want):
+                if c.dtype == E4M3:
+                    for x in (c, ones):
+                        x.view(torch.uint8)[b, :, L:] = 0x7f
+                        x.view(torch.uint8)[b, :, 16:16 * first] = 0x7f
+                else:
+                    c[b, :, 1:first] = odd[which]
+                    c[b, :, (L - 1) // 16 + 1:] = odd[which]
+                    ones[b, :, 1:first] = 1.0
+        q = _queries(2, 8, T, g, gpu)
+        at = torch.tensor(lengths, dtype=torch.int32, device=gpu)
+        got = shadowkv.kv8_attn(q, *caches, at, block=16, window=window, sinks=sinks)
+        _check_attn(q, want, lengths, None, 16, window, sinks, got=got)
+        # seen by the first queries and not by the last ones (from T = 17 on)
+        caches = _filled(2, 2, cap, 16, g, gpu)
+        caches[2 + which % 2][:, :, (231 - T - 14) // 16] = math.nan
+        got = shadowkv.kv8_attn(q, *caches, at, block=16, window=window, sinks=sinks).cpu()
+        for b, L in enumerate(lengths):
+            j = torch.arange(L) // 16 == (231 - T - 14) // 16
+            hit = _see(T, T, L, window, sinks)[:, j].any(1)
+            assert hit.any() or b == 0
+            assert torch.equal(got[b].isnan().all(-1), hit.unsqueeze(1).expand(T, 8)), (which, b)
+            assert torch.equal(got[b].isnan().any(-1), hit.unsqueeze(1).expand(T, 8)), (which, b)
+
+
+@pytest.mark.parametrize("T", [1, 12, 50])
+def test_attn_any_scales(gpu, T):
+    """Scales that no write makes (no powers of two, zeros) and factors of the scores that are zero or negative."""
+    _say(f"kv8_attn any scales T={T}")
+    g = torch.Generator().manual_seed(T)
+    caches = _filled(2, 2, 400, 32, g, gpu)
+    q = _queries(2, 8, T, g, gpu)
+    for factor in (0.0, -0.05, 0.3):
+        _check_attn(q, caches, [400, 333], None, 32, scale=factor)
+    for s in caches[2:]:
+        s.mul_((0.6 + torch.rand(s.shape, generator=g)).to(gpu))
+    caches[3][0, 1, 2] = 0.0
+    caches[2][1, 0, 3] = 0.0
+    _check_attn(q, caches, [400, 333], None, 32)
+    _check_attn(q, caches, [400, 333], [T, T // 2], 32, 100, 40)
+
+
+def test_attn_layouts(gpu):
+    """Queries and caches of other strides: heads and tokens in any order, a key and its value side by side, one kv
+    head's cache for all, a capacity of one, rows that start off 16 bytes."""
+    _say("kv8_attn layouts")
+    g = torch.Generator().manual_seed(21)
+    for T in (1, 6, 45):
+        for order in ("bsh", "slice"):
+            _check_attn(_queries(2, 6, T, g, gpu), _filled(2, 3, 333, 16, g, gpu, order), [333, 150], None, 16)
+        side = _garbage((2, 3, 200, 2, D), g).to(gpu)
+        scales = torch.ones(2, 3, 7, 2, device=gpu)
+        caches = [side[:, :, :, 0], side[:, :, :, 1], scales[..., 0].contiguous(), scales[..., 1].contiguous()]
+        k, v = _rows(2, 3, 200, g, gpu, 0.3), _rows(2, 3, 200, g, gpu, 0.3)
+        shadowkv.kv8_write(k, v, *caches, torch.zeros(2, dtype=torch.int32, device=gpu), block=32)
+        _check_attn(_queries(2, 6, T, g, gpu), caches, [200, 64], None, 32)
+        one = [c[:, :1].expand(-1, 3, *[-1] * (c.dim() - 2)) for c in caches]
+        _check_attn(_queries(2, 6, T, g, gpu), one, [200, 64], None, 32)
+        flat = torch.randn(2 * 6 * T * D + 1, generator=g).to(BF16).to(gpu)[1:].view(2, 6, T, D)
+        _check_attn(flat, caches, [200, 64], None, 32)
+        _check_attn(_queries(2, 6, T, g, gpu), _filled(2, 3, 1, 16, g, gpu), [1, 0], None, 16)
+
+
 def test_attn_long_and_uneven(gpu):
     """A batch of one long and many short sequences (chunks of several groups to a wave, 70 sequences over two
     passes of the plan), and a few tokens of long ones (keys split over workgroups)."""
