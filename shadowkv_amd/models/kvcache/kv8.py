@@ -1,0 +1,110 @@
+"""A full KV cache in 8 bits on the device, for layers that attend to everything (or to a sliding window and the
+sequence's first tokens) rather than to a selection. No reference counterpart.
+
+Keys and values are e4m3 codes [layers, B, H, max_length, 128] with one float32 power of two per block of
+`block` tokens and head (shadowkv.kv8_write, kv8_attn, kv8_read): half the bytes of bf16, quantised as they are
+written. The lengths live on the device and the step advances them itself, at layer 0, so prompts of different
+lengths share a batch and a captured step stays valid as the cache grows.
+"""
+from __future__ import annotations
+
+import torch
+
+from ...kernels import shadowkv
+from .base import KVCacheBase
+
+
+class KV8Cache(KVCacheBase):
+    """Every layer's keys and values in 8 bits; a step updates the layers in order, from layer 0."""
+
+    def __init__(self, config, batch_size: int = 1, max_length: int = 32 * 1024, device: str = "cuda:0",
+                 dtype=torch.bfloat16, block: int = 64, window: int | None = None, sinks: int = 0) -> None:
+        self.config = config
+        self.batch_size = batch_size
+        self.max_length = max_length
+        self.device = device
+        self.dtype = dtype
+        self.num_key_value_groups = config.num_attention_heads // config.num_key_value_heads
+        self.head_dim = config.hidden_size // config.num_attention_heads
+        self.num_attention_heads = config.num_attention_heads
+        self.num_key_value_heads = config.num_key_value_heads
+        self.num_layers = config.num_hidden_layers
+        if self.head_dim != 128 or dtype != torch.bfloat16:
+            raise ValueError(f"KV8Cache takes bf16 heads of 128 dims, not {dtype} of {self.head_dim}")
+        if block not in shadowkv.KV8_BLOCKS:
+            raise ValueError(f"block={block} must be one of {shadowkv.KV8_BLOCKS}")
+        if not 1 <= max_length <= shadowkv.KV8_MAX_TOKENS:
+            raise ValueError(f"max_length={max_length} must be 1 to {shadowkv.KV8_MAX_TOKENS}")
+        if (window is not None and window < 1) or sinks < 0 or (sinks and window is None):
+            raise ValueError(f"window={window} sinks={sinks} (a window of at least 1; sinks need one)")
+        self.block, self.window, self.sinks = block, window, sinks
+
+        shape = (self.num_layers, batch_size, self.num_key_value_heads, max_length, self.head_dim)
+        blocks = (max_length + block - 1) // block
+        # What no sequence holds is never used, so the codes need no clearing, here or in clear().
+        self.k8, self.v8 = (torch.empty(shape, dtype=torch.float8_e4m3fn, device=device) for _ in range(2))
+        self.k_scale, self.v_scale = (torch.empty(*shape[:3], blocks, dtype=torch.float32, device=device)
+                                      for _ in range(2))
+        self.lengths = torch.zeros(batch_size, dtype=torch.int32, device=device)  # tokens held, new ones among them
+        self.start = torch.zeros(batch_size, dtype=torch.int32, device=device)  # where this step's tokens begin
+        self.counts = None  # this step's tokens of each sequence, or None: all that were given
+        self.incoming = 0
+        self.kv_offset = 0  # the host's bound on the longest sequence: padded rows count
+
+    def print_stats(self):
+        seen = "all" if self.window is None else f"{self.window} + {self.sinks}"
+        print(f"KV8 | block {self.block} | seen {seen} | cached {self.kv_offset} of {self.max_length}")
+
+    def check_capacity(self, incoming: int = 1):
+        if self.kv_offset + incoming > self.max_length:
+            raise RuntimeError(f"cache capacity exhausted: {self.kv_offset} of {self.max_length} tokens held, "
+                               f"{incoming} new; construct the cache with a larger max_length")
+
+    def advance(self, incoming: int = 1):
+        """Host bookkeeping of one step (the device lengths advance inside the step)."""
+        self.kv_offset += incoming
+
+    def update_kv_cache(self, new_k_cache: torch.Tensor, new_v_cache: torch.Tensor, layer_idx: int,
+                        counts: torch.Tensor | None = None):
+        """Append the new tokens [B, H, T, 128] of one layer: the first counts[b] rows of each sequence (device int32
+        [B]; all T without it, and given at layer 0 for the whole step)."""
+        incoming = new_k_cache.shape[-2]
+        if layer_idx == 0:
+            self.check_capacity(incoming)
+            self.start.copy_(self.lengths)
+            self.lengths.add_(incoming if counts is None else counts.clamp(0, incoming))
+            self.counts, self.incoming = counts, incoming
+        elif incoming != self.incoming:
+            raise ValueError(f"layer {layer_idx} got {incoming} tokens in a step of {self.incoming}")
+        shadowkv.kv8_write(new_k_cache, new_v_cache, self.k8[layer_idx], self.v8[layer_idx], self.k_scale[layer_idx],
+                           self.v_scale[layer_idx], self.start, self.counts, block=self.block)
+        if layer_idx == self.num_layers - 1:
+            self.advance(incoming)
+
+    def attend(self, query_states: torch.Tensor, layer_idx: int) -> torch.Tensor:
+        """Attention of this step's queries [B, Hq, T, 128] over the layer, their own keys in it -> [B, T, Hq, 128];
+        zeros past counts[b]."""
+        if query_states.shape[-2] != self.incoming:
+            raise ValueError(f"{query_states.shape[-2]} queries in a step of {self.incoming} tokens")
+        return shadowkv.kv8_attn(query_states, self.k8[layer_idx], self.v8[layer_idx], self.k_scale[layer_idx],
+                                 self.v_scale[layer_idx], self.lengths, self.counts, block=self.block,
+                                 window=self.window, sinks=self.sinks)
+
+    def get_kv(self, layer_idx: int, start: int, rows: int):
+        """Rows [start, start + rows) of every sequence of the layer as bf16 keys and values [B, H, rows, 128] (what
+        was written, rounded to the cache's codes; rows behind a sequence's last are arbitrary)."""
+        return (shadowkv.kv8_read(self.k8[layer_idx], self.k_scale[layer_idx], start, rows, block=self.block),
+                shadowkv.kv8_read(self.v8[layer_idx], self.v_scale[layer_idx], start, rows, block=self.block))
+
+    def H2D(self):
+        torch.cuda.synchronize(self.device)  # all of it is on the device already
+
+    def clear(self):
+        self.lengths.zero_()
+        self.start.zero_()
+        self.counts = None
+        self.incoming = 0
+        self.kv_offset = 0
+
+    def get_kv_len(self):
+        return self.kv_offset
