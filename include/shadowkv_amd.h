@@ -624,11 +624,12 @@ int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_stride_h, i
  * window > 0 only those with j > p - window or j < sinks:
  *   out[b, t, hq, :] = sum_j exp(scale q[b, hq, t] . k_j) v_j / sum_j exp(scale q[b, hq, t] . k_j)
  * over them, of kv head hq / (q_heads / kv_heads); zeros for a query that sees nothing (p < 0) and for t >= n_b.
- * Keys and values that a query does not see do not reach it, whatever they hold. Scores, probabilities and sums
- * in fp32, out [batch, rows, q_heads, 128] bf16 (contiguous, 16-byte aligned). q: rows of 128 bf16 at
- * q + b*q_stride_b + hq*q_stride_h + t*q_stride_t, multiples of 8 elements, 16-byte aligned. lengths and counts
- * are read when the kernels run. workspace: skv_kv8_attn_workspace_bytes bytes (0 for some sizes, and for bad
- * ones), 16-byte aligned, overwritten. */
+ * Keys and values that a query does not see do not reach it, whatever they and their scales hold. Scores and sums in
+ * fp32; with more than 32 rows * q_heads / kv_heads and value scales that are powers of two within 2^12 of one another,
+ * probabilities enter their product in f16, else with 16 significant bits. out [batch, rows, q_heads, 128] bf16
+ * (contiguous, 16-byte aligned). q: rows of 128 bf16 at q + b*q_stride_b + hq*q_stride_h + t*q_stride_t, multiples of
+ * 8 elements, 16-byte aligned. c_stride_s at most 2^24. lengths and counts are read when the kernels run. workspace:
+ * skv_kv8_attn_workspace_bytes bytes (0 for some sizes, and for bad ones), 16-byte aligned, overwritten. */
 int64_t skv_kv8_attn_workspace_bytes(int batch_size, int q_heads, int kv_heads, int rows, int cap, int window,
                                      int sinks);
 int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_stride_h, int64_t q_stride_t, const uint8_t* k8,

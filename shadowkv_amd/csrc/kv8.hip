@@ -6,7 +6,9 @@
 // none of its 4 significant bits, code * scale is exact in bf16, and rows encoded again under a larger scale
 // change only where they become subnormal.
 //
-// Bound: HBM bytes (written rows 2 + 1 per element, read rows 1 + 2); a decoded token is a launch.
+// Bound: HBM bytes (written rows 2 + 1 per element, read rows 1 + 2); a decoded token is a launch. Measured (MI355X, 8
+// heads): 122880 tokens written in 140 us, 5.4 TB/s (a large copy has 4.7); 100003 rows read in 63, 4.9 TB/s; a
+// token of each of 8 sequences written in 4.4 on the device (12.8 a call from Python).
 #include "skv_common.h"
 
 namespace {
@@ -279,8 +281,9 @@ extern "C" int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_
   }
   const int chunk = chunk_ids ? chunk_size : 1;
   ReadArgs a{codes, scale, c_stride_b, c_stride_h, c_stride_s, s_stride_b, s_stride_h, chunk_ids, out, start, heads,
-             cap, block, chunk, static_cast<int>((static_cast<int64_t>(cap) + chunk - 1) / chunk), rows, static_cast<int>(groups)};
-  hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0, static_cast<hipStream_t>(stream),
-                     a);
+             cap, block, chunk, static_cast<int>((static_cast<int64_t>(cap) + chunk - 1) / chunk), rows,
+             static_cast<int>(groups)};
+  hipLaunchKernelGGL(read_kernel, dim3(static_cast<unsigned>(grid)), dim3(kThreads), 0,
+                     static_cast<hipStream_t>(stream), a);
   return skv_check_launch(what);
 }

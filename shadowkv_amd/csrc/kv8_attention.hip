@@ -6,9 +6,10 @@
 // over the keys j <= p of the query's position p = length_b - n_b + t, with a window w only those with j > p - w
 // or j < sinks. A query that sees nothing, or is padding (t >= n_b), gets zeros. Codes become bf16 (exactly) on
 // their way into the matrix cores; a key block's scale multiplies its scores and a value block's scale its
-// probabilities, so no dequantised row is ever formed. Scores, probabilities and sums are fp32; a probability
+// probabilities, so no dequantised row is ever formed. Scores, probabilities and sums are fp32. A probability
 // enters the product with the values as two bf16 parts (16 significant bits, an error of 2^-16 where the output's
-// one rounding is 2^-9).
+// one rounding is 2^-9); with many rows, where the matrix cores are the bound, as one f16 (11 bits, 2^-12, and the
+// sum that divides the result takes the same rounded ones), wherever f16 holds the values exactly.
 #include <algorithm>
 #include <cmath>
 #include <type_traits>
@@ -148,7 +149,9 @@ __device__ __forceinline__ float sum_of_rows(float x) {
 // of four waves that take its groups of 32 keys in turn, straight from memory into registers: S^T = K Q^T on
 // v_mfma_f32_16x16x32_bf16 (a row of the queries a column) leaves a lane with 8 keys' scores of one row, which is the
 // second operand of O^T = V^T P^T, whose first is the lane's 8 tokens of one dim: neither probabilities nor
-// values cross lanes.
+// values cross lanes. Measured (MI355X, 4 query heads on each of 8 kv heads): 8 sequences of 122880 tokens 306 us, 6.6
+// TB/s; 24 windows of 8192 keys and 64 sinks 74 us, 5.3 TB/s; 5 tokens each of 4 sequences of up to 30011 42 us, 3.7
+// TB/s (two tiles of rows leave two waves a SIMD, and the conversions and exponentials 20 us of it).
 constexpr int kGroup = 32;
 constexpr int kGroupShift = 5;
 constexpr int kMinGroups = 8;   // a chunk's groups of 32 keys, at least
@@ -158,9 +161,9 @@ constexpr int target_chunks(int64_t rows) { return rows <= 8 ? 2048 : 1024; }
 constexpr int kOutLd = kD + 4;
 // Groups that a sequence's rows can see (by the capacity and the window) up to which one workgroup of 16 waves (8 for
 // two tiles of rows) takes them all, in one launch, rather than chunks and a join: a window of 1024 keys with sinks,
-// its ends inside a group, or twice that where the sequences fill half of the chip (MI355X, us in a graph, 4 query heads
-// on each of 8 kv heads, chunks / whole: 1 sequence of 512 keys 10.0 / 7.6, 1024 9.9 / 10.1 and a launch less from the
-// host, 2048 10.0 / 15.8; 24 sequences of 1024 16.4 / 11.8, 2048 26.1 / 20.2).
+// its ends inside a group, or twice that where the sequences fill half of the chip (MI355X, us in a graph, 4 query
+// heads on each of 8 kv heads, chunks / whole: 1 sequence of 512 keys 10.0 / 7.6, 1024 9.9 / 10.1 and a launch less
+// from the host, 2048 10.0 / 15.8; 24 sequences of 1024 16.4 / 11.8, 2048 26.1 / 20.2).
 constexpr int whole_groups(int tiles, int64_t rows_of_kv) { return (rows_of_kv >= 128 ? 72 : 36) / tiles; }
 
 struct Chunk {
@@ -383,7 +386,8 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int r = 0; r < 4; r += 2) {
-          const float p0 = __builtin_amdgcn_exp2f(s[y][u][r] - ref), p1 = __builtin_amdgcn_exp2f(s[y][u][r + 1] - ref);
+          const float p0 = __builtin_amdgcn_exp2f(s[y][u][r] - ref);
+          const float p1 = __builtin_amdgcn_exp2f(s[y][u][r + 1] - ref);
           l[y] += p0 + p1;
           uint32_t first, second;
           two_parts(p0 * vf[y][u], p1 * vf[y][u], first, second);
@@ -406,7 +410,8 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
           for (int y = 0; y < kTiles; ++y)
             o[y][4 * half + e] =
                 __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, vt[e]),
-                                                        __builtin_bit_cast(bf16x8, part[y][x]), o[y][4 * half + e], 0, 0, 0);
+                                                        __builtin_bit_cast(bf16x8, part[y][x]), o[y][4 * half + e], 0,
+                                                        0, 0);
     }
   }
 
@@ -449,8 +454,8 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
         const float inv = query && lsum != 0.f ? 1.f / lsum : 0.f;  // (nothing seen: zeros)
         const u32x2 out = {skv::f2bf2(sum[0] * inv, sum[1] * inv), skv::f2bf2(sum[2] * inv, sum[3] * inv)};
         const int t = row / G;
-        *reinterpret_cast<u32x2*>(a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H * G + h * G + row - t * G) * kD + d) =
-            query ? out : u32x2{0u, 0u};
+        const int64_t at = (static_cast<int64_t>(b) * a.T + t) * a.H * G + h * G + row - t * G;
+        *reinterpret_cast<u32x2*>(a.out + at * kD + d) = query ? out : u32x2{0u, 0u};
         continue;
       }
       *reinterpret_cast<f32x4*>(a.ws_o + (row0 + row) * kD + d) = query ? sum : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -514,14 +519,18 @@ __global__ void __launch_bounds__(256) few_join_kernel(Args a) {
 // More rows.
 //
 // Bound: the matrix cores (with few rows, HBM). The rows of a kv head are its queries' heads together, row
-// t * G + g, so that a tile of keys serves all of them. A workgroup of four waves owns 128 rows (32 a wave, a row
-// a lane) and walks the tiles of 64 keys that any of them sees, or a share of them where there are too few rows to
-// fill the chip. Keys and values are read once a tile, turned into bf16 (the values transposed) by the threads
-// that read them, and shared through LDS, the next tile on its way meanwhile.
+// t * G + g, so that a tile of keys serves all of them. A workgroup of four waves (eight) owns 128 (256) rows, 32 a
+// wave, a row a lane, and walks the tiles of 64 keys that any of them sees, or a share of them where there are too few
+// rows to fill the chip. Keys and values are read once a tile, turned into 16 bits (the values transposed) by the
+// threads that read them, and shared through LDS, the next tile on its way meanwhile. Measured (MI355X): 8192 causal
+// tokens of 32 heads over 8, 540 us, 1.02 PFLOP/s where a large bf16 GEMM has 1.22; 2048 tokens behind up to 31285
+// others, 16 heads on each of 2 kv heads, a window of 8192, two sequences, 520 us, 0.93 PFLOP/s. Of a tile's time,
+// the matrix instructions of a wave take 1024 cycles, as many as the four SIMDs' reads of their operands take of LDS,
+// and the vector work (conversions, exponentials, maximum) 870, which hides behind the former only in part; the clock
+// is at 1.9 of 2.4 GHz under this load.
 constexpr int kTile = 64;
 constexpr int kTileShift = 6;
 constexpr int kRowsWave = 32;
-constexpr int kRowsTile = 4 * kRowsWave;
 
 // 16-byte chunk c (8 dims) of key row r of a tile in LDS, and chunk (group of 16 keys, half of its order, dim).
 __device__ __forceinline__ int k_at(int r, int c) { return r * 16 + (c ^ (r & 15)); }
@@ -553,11 +562,16 @@ constexpr int kRaise = 7;
 // A probability is at most 2^(kRaise + kSlack), below f16's largest: kSlack is how far a score may pass the reference.
 constexpr float kSlack = 8.f;
 
-__global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
+// kWaves: 4, two workgroups to a CU, or 8, one.
+template <int kWaves>
+__global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
+  constexpr int kRowsTile = kWaves * kRowsWave;
+  constexpr int kKeyLoads = 8 / kWaves;   // of 16 bytes of a key's row that a thread carries
+  constexpr int kValueDims = 16 / kWaves;  // that it carries of the values of 8 tokens
   __shared__ u32x4 kt[2][kTile * 16], vt[2][kTile * 16];
   // Values that are NaN, by (buffer, wave that carries them): whether there are any, and each dim's keys as bits.
-  __shared__ int odd_lds[2][4];
-  __shared__ uint32_t odd_keys[2][4][kD];
+  __shared__ int odd_lds[2][kWaves];
+  __shared__ uint32_t odd_keys[2][kWaves][kD];
   __shared__ int vexp[3];  // largest and smallest exponent of the value blocks' scales, whether one is no power of two
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -593,6 +607,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     x.query = x.row < R && x.t < n;
     return x;
   };
+  // A wave of rows past the last, or of padding: it carries its share of the tiles, and no more.
+  const bool idle = r0 + wave * kRowsWave >= min(R, n * G);
   u32x4 qf[8];
   {
     const Row x = row_of(threadIdx.x & 31);
@@ -608,13 +624,14 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   const float* ksh = a.ks + b * a.s_sb + h * a.s_sh;
   const float* vsh = a.vs + b * a.s_sb + h * a.s_sh;
 
-  // A thread carries 32 bytes of a key row, and four dims of the values of 8 tokens: half of a group of 16, a wave's,
-  // in the order of the keys in the scores' registers. Rows behind the sequence's end are out of the buffer's bounds
-  // and come as zeros, whatever lies there.
+  // A thread carries 32 bytes of a key row (of 8 waves 16), and four dims (two) of the values of 8 tokens: half of a
+  // group of 16, in the order of the keys in the scores' registers; a group is a wave's (two waves', a half each). Rows
+  // behind the sequence's end are out of the buffer's bounds and come as zeros, whatever lies there.
   const int stride = static_cast<int>(a.c_ss);
   struct Lane {
-    int li, half, krow, kpart, kmine, vmine;
+    int li, half, krow, kpart, kmine, vmine, vhalf, vdim;
   };
+  const int vgroup = kWaves == 4 ? wave : wave >> 1;
   // (made anew where a walk begins, from a thread id that the compiler takes for another one: what hangs on it would
   // else be held in registers from walk to walk)
   auto own_lane = [&]() __attribute__((always_inline)) {
@@ -623,38 +640,44 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     Lane x;
     x.li = tid & 31;
     x.half = (tid >> 5) & 1;
-    x.krow = tid >> 2;
-    x.kpart = tid & 3;
-    x.kmine = x.krow * stride + 32 * x.kpart;
-    x.vmine = (16 * wave + 4 * x.half) * stride + 4 * x.li;
+    x.krow = tid / kWaves;
+    x.kpart = tid % kWaves;
+    x.kmine = x.krow * stride + 16 * kKeyLoads * x.kpart;
+    x.vhalf = kWaves == 4 ? x.half : wave & 1;
+    x.vdim = kValueDims * (kWaves == 4 ? x.li : tid & 63);
+    x.vmine = (16 * vgroup + 4 * x.vhalf) * stride + x.vdim;
     return x;
   };
   constexpr int kDw3 = 0x00020000;  // buffer resource word 3 (gfx9)
   auto tile_rows = [&](const uint8_t* base, int tile) __attribute__((always_inline)) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + static_cast<int64_t>(tile) * kTile * a.c_ss), 0,
-                                             min(len - tile * kTile - 1, kTile - 1) * stride + kD, kDw3);
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(base + static_cast<int64_t>(tile) * kTile * a.c_ss), 0,
+        min(len - tile * kTile - 1, kTile - 1) * stride + kD, kDw3);
   };
-  u32x4 kheld[2];
+  u32x4 kheld[kKeyLoads];
   uint32_t vheld[8];
   auto fetch_keys = [&](const Lane& x, __amdgpu_buffer_rsrc_t src) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) kheld[c] = __builtin_amdgcn_raw_buffer_load_b128(src, x.kmine, 16 * c, 0);
+    for (int c = 0; c < kKeyLoads; ++c) kheld[c] = __builtin_amdgcn_raw_buffer_load_b128(src, x.kmine, 16 * c, 0);
   };
   auto fetch_values = [&](const Lane& x, __amdgpu_buffer_rsrc_t src) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      vheld[e] = __builtin_amdgcn_raw_buffer_load_b32(src, x.vmine, ((e & 3) + 8 * (e >> 2)) * stride, 0);
+    for (int e = 0; e < 8; ++e) {
+      const int at = ((e & 3) + 8 * (e >> 2)) * stride;
+      if constexpr (kWaves == 4) vheld[e] = __builtin_amdgcn_raw_buffer_load_b32(src, x.vmine, at, 0);
+      else vheld[e] = __builtin_amdgcn_raw_buffer_load_b16(src, x.vmine, at, 0);
+    }
+  };
+  auto place_chunk = [&](const Lane& x, int buf, int c) __attribute__((always_inline)) {
+    kt[buf][k_at(x.krow, 2 * kKeyLoads * x.kpart + c)] =
+        __builtin_bit_cast(u32x4, bf16_of(kheld[c >> 1][2 * (c & 1)], kheld[c >> 1][2 * (c & 1) + 1]));
   };
   auto place_keys = [&](const Lane& x, int buf) __attribute__((always_inline)) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      kt[buf][k_at(x.krow, 4 * x.kpart + 2 * c)] = __builtin_bit_cast(u32x4, bf16_of(kheld[c][0], kheld[c][1]));
-      kt[buf][k_at(x.krow, 4 * x.kpart + 2 * c + 1)] = __builtin_bit_cast(u32x4, bf16_of(kheld[c][2], kheld[c][3]));
-    }
+    for (int c = 0; c < 2 * kKeyLoads; ++c) place_chunk(x, buf, c);
   };
-  auto put_values = [&](const Lane& x, const u32x4 (&o)[4], int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) vt[buf][v_at(wave, x.half, 4 * x.li + e)] = o[e];
+  auto put_value = [&](const Lane& x, const u32x4& o, int buf, int e) __attribute__((always_inline)) {
+    vt[buf][v_at(vgroup, x.vhalf, x.vdim + e)] = o;
   };
   // The block of a tile's group of 16 keys.
   auto block_of = [&](int tile, int group) __attribute__((always_inline)) {
@@ -733,7 +756,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
   // at the smallest, 2^-126, are zeros beside any other).
   if (threadIdx.x < 3) vexp[threadIdx.x] = threadIdx.x == 0 ? 1 : threadIdx.x == 1 ? 255 : 0;
   __syncthreads();
-  for (int i = 4 * i0 + threadIdx.x; i < 4 * i1; i += 256) {
+  for (int i = 4 * i0 + threadIdx.x; i < 4 * i1; i += 64 * kWaves) {
     const uint32_t v = __float_as_uint(vsh[block_of(seen.at(i >> 2), i & 3)]);
     const int e = static_cast<int>(v >> 23);
     if (v > 0x00800000u) {
@@ -753,15 +776,20 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     return __uint_as_float(static_cast<uint32_t>(max(static_cast<int>(v >> 23) - vtop + 127 + kRaise, 1)) << 23);
   };
 
+  // Part y of the values, in f16: two tokens' pairs of two dims.
+  auto place_pairs = [&](const Lane& x, int buf, int y, float factor, u32x4 (&o)[2]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int e = 2 * (y & 1); e < 2 * (y & 1) + 2; ++e)
+      f16_pair(vheld[2 * e], vheld[2 * e + 1], factor, y >> 1, e, o[0], o[1]);
+    if (y & 1)
+#pragma unroll
+      for (int z = 0; z < 2; ++z) put_value(x, o[z], buf, 2 * (y >> 1) + z);
+  };
   auto place_f16 = [&](const Lane& x, int tile, int buf) __attribute__((always_inline)) {
-    u32x4 o4[4];
-    const float factor = value_factor(scale_at(vsh, block_of(tile, wave)));
+    u32x4 o[2];
+    const float factor = value_factor(scale_at(vsh, block_of(tile, vgroup)));
 #pragma unroll
-    for (int y = 0; y < 2; ++y)
-#pragma unroll
-      for (int e = 0; e < 4; ++e)
-        f16_pair(vheld[2 * e], vheld[2 * e + 1], factor, y, e, o4[2 * y], o4[2 * y + 1]);
-    put_values(x, o4, buf);
+    for (int y = 0; y < kValueDims; ++y) place_pairs(x, buf, y, factor, o);
   };
 
   // Tiles that every row sees whole, values and probabilities in f16, one product. Tile i's probabilities and their
@@ -778,8 +806,8 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base + min(tile, end) * tile_bytes), 0,
                                                (kTile - 1) * stride + kD, kDw3);
     };
-    // The factors of a tile's groups of 16 keys in a lane each: the keys' in lanes 0 to 3, the values' in 4 to 7. Of tiles
-    // i and i + 1, and the scales of i + 2.
+    // The factors of a tile's groups of 16 keys in a lane each: the keys' in lanes 0 to 3, the values' in 4 to 7. Of
+    // tiles i and i + 1, and the scales of i + 2.
     float factors[2], scales;
     const float* own_scales = g.li & 4 ? vsh : ksh;
     auto fetch_scales = [&](int tile) __attribute__((always_inline)) {
@@ -791,6 +819,11 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     };
     auto lane_factor = [&](float held, int which) __attribute__((always_inline)) {
       return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), which));
+    };
+    auto next_factors = [&](int i) __attribute__((always_inline)) {
+      factors[0] = factors[1];
+      factors[1] = factors_of(scales);
+      scales = fetch_scales(i + 3);
     };
     // One tile: its scores in s, the next one's into sn (past the last, the last one's again). Keys i are in kt[par],
     // values in vt[par]. 32 slices of a matrix instruction each (16 of the next scores, 16 of this product), its
@@ -810,7 +843,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       float kf[4];
 #pragma unroll
       for (int q = 0; q < 4; ++q) kf[q] = lane_factor(factors[0], q);
-      const float factor = lane_factor(factors[1], 4 + wave);
+      const float factor = lane_factor(factors[1], 4 + vgroup);
       float mx = -INFINITY, ref = 0.f;
       auto largest_of = [&](int q) __attribute__((always_inline)) {
         mx = fmaxf(mx, max8(s[q >> 1], 8 * (q & 1)) * kf[q]);
@@ -835,35 +868,25 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
         if (j < 29) operand(j + 3);
         if (j < 16)
           sn[j & 1] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[j & 3]),
-                                                              __builtin_bit_cast(bf16x8, qf[j >> 1]), sn[j & 1], 0, 0, 0);
+                                                              __builtin_bit_cast(bf16x8, qf[j >> 1]), sn[j & 1], 0, 0,
+                                                              0);
         else
           o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f[j & 3]),
                                                             __builtin_bit_cast(f16x8, part[(j - 16) >> 2]), o[j & 3], 0,
                                                             0, 0);
+        // (vector work, evenly: the maximum and the reference, 16 pairs of probabilities, each before the product that
+        // takes it, and between those the tiles on their way)
+        constexpr int kPair[32] = {-1, -1, -1, -1, 0, 1, -1, 2, 3, -1, 4, 5, -1, 6, 7, -1,
+                                   8, 9, -1, 10, 11, -1, 12, 13, -1, 14, 15, -1, -1, -1, -1, -1};
         if (j < 3) largest_of(j + 1);
         else if (j == 3) ref = refer(largest_half(mx));
-        else if (j < 20) probabilities((j - 4) >> 2, j & 3);
-        else if (j < 24) {
-          const int c = j - 20;
-          kt[par][k_at(g.krow, 4 * g.kpart + c)] = __builtin_bit_cast(
-              u32x4, bf16_of(kheld[c >> 1][2 * (c & 1)], kheld[c >> 1][2 * (c & 1) + 1]));
-        } else if (j < 28) {  // two tokens' pairs of two dims
-          const int y = (j - 24) >> 1;
-#pragma unroll
-          for (int e = 2 * (j & 1); e < 2 * (j & 1) + 2; ++e)
-            f16_pair(vheld[2 * e], vheld[2 * e + 1], factor, y, e, x[0], x[1]);
-          if (j & 1)
-#pragma unroll
-            for (int z = 0; z < 2; ++z) vt[par ^ 1][v_at(wave, g.half, 4 * g.li + 2 * y + z)] = x[z];
-        } else if (j == 28) {
-          fetch_keys(g, whole_rows(kh, i + 3));
-        } else if (j == 29) {
-          fetch_values(g, whole_rows(vh, i + 2));
-        } else if (j == 30) {
-          factors[0] = factors[1];
-          factors[1] = factors_of(scales);
-          scales = fetch_scales(i + 3);
-        }
+        else if (kPair[j] >= 0) probabilities(kPair[j] >> 2, kPair[j] & 3);
+        else if (j <= 15 && j % 3 == 0 && j / 3 - 2 < 2 * kKeyLoads) place_chunk(g, par, j / 3 - 2);
+        else if (j == 18) fetch_keys(g, whole_rows(kh, i + 3));
+        else if (j == 21 || j == 24) place_pairs(g, par ^ 1, j / 3 - 7, factor, x);
+        else if ((j == 27 || j == 28) && kValueDims == 4) place_pairs(g, par ^ 1, j - 25, factor, x);
+        else if (j == 29) fetch_values(g, whole_rows(vh, i + 2));
+        else if (j == 30) next_factors(i);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
@@ -878,11 +901,28 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
     fetch_keys(g, whole_rows(kh, from + 2));
     fetch_values(g, whole_rows(vh, from + 1));
     __syncthreads();
-    f32x16 sa[2], sb[2];
-    scores(g, 0, sa);
     factors[0] = factors_of(fetch_scales(from));
     factors[1] = factors_of(fetch_scales(from + 1));
     scales = fetch_scales(from + 2);
+    if (idle) {  // wave-uniform
+      for (int i = from; i <= end; ++i) {
+        barrier_lds();
+        const int par = (i - from) & 1;
+        const float factor = lane_factor(factors[1], 4 + vgroup);
+        u32x4 x[2];
+#pragma unroll
+        for (int c = 0; c < 2 * kKeyLoads; ++c) place_chunk(g, par, c);
+#pragma unroll
+        for (int y = 0; y < kValueDims; ++y) place_pairs(g, par ^ 1, y, factor, x);
+        fetch_keys(g, whole_rows(kh, i + 3));
+        fetch_values(g, whole_rows(vh, i + 2));
+        next_factors(i);
+      }
+      return;
+    }
+    f32x16 sa[2], sb[2];
+    scores(g, 0, sa);
+    asm volatile("s_nop 15\n\ts_nop 7" : "+v"(sa[0]), "+v"(sa[1]));  // (their first reader is max8's asm)
     for (int i = from;;) {
       step(std::integral_constant<int, 0>{}, i, sa, sb);
       if (++i > end) break;
@@ -909,14 +949,15 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       for (int e = 0; e < 8; ++e) {
         const uint32_t f = nan_bytes(vheld[e]);
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          if (f & (0x80u << (8 * y))) atomicOr(&keys[4 * x.li + y], 1u << (4 * x.half + (e & 3) + 8 * (e >> 2)));
+        for (int y = 0; y < kValueDims; ++y)
+          if (f & (0x80u << (8 * y))) atomicOr(&keys[x.vdim + y], 1u << (4 * x.vhalf + (e & 3) + 8 * (e >> 2)));
         vheld[e] &= ~((f >> 7) * 0xffu);
       }
     }
     u32x4 o4[4];
     transpose_bf16(vheld, o4);
-    put_values(x, o4, buf);
+#pragma unroll
+    for (int e = 0; e < kValueDims; ++e) put_value(x, o4[e], buf, e);
   };
   auto walk = [&](auto f16, int from, int to) __attribute__((always_inline)) {
     constexpr bool kF16 = decltype(f16)::value;
@@ -937,6 +978,7 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
         fetch_keys(g, tile_rows(kh, seen.at(i + 1)));
         fetch_values(g, tile_rows(vh, seen.at(i + 1)));
       }
+      if (idle) continue;  // wave-uniform
       f32x16 s[2];
       float kf[4];
       scores(g, buf, s);
@@ -950,12 +992,13 @@ __global__ void __launch_bounds__(256, 2) rows_kernel(Args a) {
       hide(g, p, tile, s);  // (behind the factors: a hidden block's scale may be anything)
       const float ref = refer(largest(s));
       if constexpr (!kF16) {
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < kWaves; ++q) {
           // A value that is NaN makes the sums of the rows that see its key NaN, and no others (in the product it
           // would: a hidden key's zero times NaN).
           if (!odd_lds[buf][q]) continue;  // the same for all
+          const int first = tile * kTile + 16 * (q / (kWaves / 4));
           uint32_t vis = 0;
-          for (int j = 0; j < 16; ++j) vis |= sees(p, tile * kTile + 16 * q + j, a.window, a.sinks) ? 1u << j : 0u;
+          for (int j = 0; j < 16; ++j) vis |= sees(p, first + j, a.window, a.sinks) ? 1u << j : 0u;
           for (int d = 0; d < 64; ++d)
             if (odd_keys[buf][q][32 * (d >> 4) + 8 * ((d & 15) >> 2) + 4 * g.half + (d & 3)] & vis) odd |= 1ull << d;
         }
@@ -1084,9 +1127,27 @@ struct Plan {
   int tiles;   // few rows: tiles of 16; 0 for more
   bool whole;  // few rows: one workgroup a (sequence, kv head)
   int64_t grid;
+  int waves;   // more: of a workgroup
   int splits, rtiles;
   int64_t parts;  // partial rows of 128 + 2 floats
 };
+
+// Tiles of 64 keys from which workgroups of 8 waves take the rows, if more than 128: a thread then turns half as many
+// codes into 16 bits, but a tile's barrier holds a whole CU (MI355X, us, 4 query heads on each of 8 kv heads, 4 waves /
+// 8: 2000 tokens of a prompt 38 / 45, 4096 110 / 105, 16384 1389 / 1365; 24 sequences' 64 tokens on 1000 keys 31.7 /
+// 31.2, on 4000 86 / 80, on 16000 334 / 311; with up to 128 rows the added waves have none: 9 tokens 50 / 56).
+constexpr int kLongTiles = 40;
+
+// Shares of a row tile's keys, of at least 4 tiles, where the workgroups alone would leave part of the chip idle: as
+// many as make the walk and the join together shortest. A workgroup walks a tile in about 1.1 us; a share's partial
+// rows, written and read, cost 1 KB each, and the join 5 us (MI355X, us, one share / as many as fit: 64 tokens on 8000
+// keys 140 / 24, on 2000 33 / 16; 1000 tokens of a prompt 21 / 39, 500 14 / 27).
+int shares(int64_t tiles, int64_t wgs, int64_t resident, double rows) {
+  const double walk = 1.1 * static_cast<double>(tiles), each = 2e-4 * rows;
+  const int64_t most = std::min<int64_t>(resident / wgs, tiles / 4);
+  const int64_t n = std::min<int64_t>(most, static_cast<int64_t>(std::sqrt(walk / each)));
+  return n > 1 && walk / static_cast<double>(n) + 5. + each * static_cast<double>(n) < walk ? static_cast<int>(n) : 1;
+}
 
 Plan plan_of(int B, int H, int G, int T, int cap, int window, int sinks) {
   Plan p{};
@@ -1109,10 +1170,12 @@ Plan plan_of(int B, int H, int G, int T, int cap, int window, int sinks) {
     p.splits = 1;
     return p;
   }
-  p.rtiles = static_cast<int>((R + kRowsTile - 1) / kRowsTile);
-  const int64_t wgs = static_cast<int64_t>(B) * H * p.rtiles;
   const int64_t tiles = (keys + kTile - 1) / kTile;
-  p.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>((512 + wgs - 1) / wgs, tiles / 4)));
+  p.waves = R > 4 * kRowsWave && tiles >= kLongTiles ? 8 : 4;
+  const int tile = p.waves * kRowsWave;
+  p.rtiles = static_cast<int>((R + tile - 1) / tile);
+  const int64_t wgs = static_cast<int64_t>(B) * H * p.rtiles;
+  p.splits = shares(tiles, wgs, 2048 / p.waves, static_cast<double>(B) * H * R);
   p.grid = wgs * p.splits;
   p.parts = p.splits > 1 ? static_cast<int64_t>(B) * H * R * p.splits : 0;
   return p;
@@ -1169,7 +1232,7 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
                   (long long)need);
     return SKV_EINVAL;
   }
-  const int threads = p.whole ? few_threads(p.tiles, true) : 256;
+  const int threads = p.whole ? few_threads(p.tiles, true) : p.tiles ? 256 : 64 * p.waves;
   const int64_t join = p.parts ? static_cast<int64_t>(batch_size) * q_heads * rows : 0;  // workgroups of it
   if (p.grid * threads >= kMaxThreads || join * 256 >= kMaxThreads) {
     skv_set_error("%s: batch=%d q_heads=%d rows=%d", what, batch_size, q_heads, rows);
@@ -1193,7 +1256,8 @@ extern "C" int skv_kv8_attn(const uint16_t* q, int64_t q_stride_b, int64_t q_str
     else hipLaunchKernelGGL((few_kernel<2, false>), g, t, 0, s, a);
     hipLaunchKernelGGL(few_join_kernel, dim3(static_cast<unsigned>(join)), t, 0, s, a);
   } else {
-    hipLaunchKernelGGL(rows_kernel, g, t, 0, s, a);
+    if (p.waves == 4) hipLaunchKernelGGL(rows_kernel<4>, g, dim3(threads), 0, s, a);
+    else hipLaunchKernelGGL(rows_kernel<8>, g, dim3(threads), 0, s, a);
     if (p.splits > 1) hipLaunchKernelGGL(rows_join_kernel, dim3(static_cast<unsigned>(join)), t, 0, s, a);
   }
   return skv_check_launch(what);

@@ -1342,7 +1342,7 @@ def kv8_attn(q, k8, v8, k_scale, v_scale, lengths, counts=None, *, block=64, sca
     and sees the keys up to its own; with a window only the last `window` of those and the first `sinks` of the
     sequence. lengths (tokens held, the new ones among them; clamped to [0, capacity]), counts: device int32 [B],
     read when the kernels run. Queries that see nothing and those past counts[b] give zeros. What a query does
-    not see may hold anything, NaN too. scale: 1 / sqrt(128) by default."""
+    not see may hold anything, NaN too, in the codes and in their scales. scale: 1 / sqrt(128) by default."""
     (B, H, cap), c_strides, s_strides, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
     _no_grad("kv8_attn", q)
     q, q_strides = _rows128(q, "q")

@@ -480,6 +480,47 @@ def test_attn_layouts(gpu):
         _check_attn(_queries(2, 6, T, g, gpu), _filled(2, 3, 1, 16, g, gpu), [1, 0], None, 16)
 
 
+@pytest.mark.parametrize("H,G,T", [(2, 4, 33), (2, 16, 9), (1, 16, 40), (1, 4, 150)])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2700, 0), (2600, 70), (3500, 1000)])
+def test_attn_many_on_long_caches(gpu, H, G, T, window, sinks):
+    """Rows beyond a workgroup of 128 on caches of thousands of keys: several shares of them, waves with no rows, the
+    ends of windows, padding, scales and layouts as elsewhere."""
+    _say(f"kv8_attn many long H={H} G={G} T={T} window={window}")
+    g = torch.Generator().manual_seed(T + G)
+    caches = _filled(2, H, 4500, 32, g, gpu, "bsh" if T == 33 else "bhs")
+    q = _queries(2, H * G, T, g, gpu)
+    _check_attn(q, caches, [4500, 2811], None, 32, window, sinks)
+    _check_attn(q, caches, [4433, T - 3], [T, T - 2], 32, window, sinks)
+    _check_attn(q, caches, [3001, 0], [1, T], 32, window, sinks)
+
+
+@pytest.mark.parametrize("window,sinks", [(None, 0), (2600, 10)])
+def test_attn_many_on_long_caches_odd(gpu, window, sinks):
+    """NaN and scales that no f16 holds together, among many rows on a long cache: seen by some, hidden from others."""
+    _say(f"kv8_attn many long odd window={window}")
+    g = torch.Generator().manual_seed(3)
+    caches = _filled(2, 2, 4000, 16, g, gpu)
+    q = _queries(2, 8, 50, g, gpu)
+    v8 = caches[1].view(torch.uint8)
+    v8[0, 0, 3960, 5] = v8[0, 1, 1375, 9] = v8[0, 1, 3, 127] = v8[0, 1, 2000, 64] = 0x7f
+    v8[1, 0, 3970:3980, 64:70] = 0xff
+    _check_attn(q, caches, [4000, 3990], None, 16, window, sinks)
+    caches = _filled(2, 2, 4000, 16, g, gpu)
+    caches[3].mul_(torch.exp2(torch.randint(-9, 9, caches[3].shape, generator=g).float()).to(gpu))
+    _check_attn(q, caches, [4000, 3977], None, 16, window, sinks)
+    caches[3].mul_((0.6 + torch.rand(caches[3].shape, generator=g)).to(gpu))
+    _check_attn(q, caches, [4000, 3977], [50, 31], 16, window, sinks)
+    caches[2][:, :, 3965 // 16] = math.nan  # seen by the last queries only
+    caches[3][:, :, 1330 // 16] = math.nan  # with the window, by the first ones only
+    got = shadowkv.kv8_attn(q, *caches, torch.tensor([4000, 3990], dtype=torch.int32, device=gpu), block=16,
+                            window=window, sinks=sinks).cpu()
+    for b, L in enumerate((4000, 3990)):
+        j = torch.arange(L) // 16
+        hit = _see(50, 50, L, window, sinks)[:, (j == 3965 // 16) | (j == 1330 // 16)].any(1)
+        assert torch.equal(got[b].isnan().all(-1), hit.unsqueeze(1).expand(50, 8))
+        assert torch.equal(got[b].isnan().any(-1), hit.unsqueeze(1).expand(50, 8))
+
+
 def test_attn_long_and_uneven(gpu):
     """A batch of one long and many short sequences (chunks of several groups to a wave, 70 sequences over two
     passes of the plan), and a few tokens of long ones (keys split over workgroups)."""
