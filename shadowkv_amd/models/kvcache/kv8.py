@@ -72,12 +72,14 @@ class KV8Cache(KVCacheBase):
         if layer_idx == 0:
             self.check_capacity(incoming)
             self.start.copy_(self.lengths)
-            self.lengths.add_(incoming if counts is None else counts.clamp(0, incoming))
-            self.counts, self.incoming = counts, incoming
         elif incoming != self.incoming:
             raise ValueError(f"layer {layer_idx} got {incoming} tokens in a step of {self.incoming}")
         shadowkv.kv8_write(new_k_cache, new_v_cache, self.k8[layer_idx], self.v8[layer_idx], self.k_scale[layer_idx],
-                           self.v_scale[layer_idx], self.start, self.counts, block=self.block)
+                           self.v_scale[layer_idx], self.start, counts if layer_idx == 0 else self.counts,
+                           block=self.block)
+        if layer_idx == 0:  # (behind the write: one that is refused leaves the lengths)
+            self.lengths.add_(incoming if counts is None else counts.clamp(0, incoming))
+            self.counts, self.incoming = counts, incoming
         if layer_idx == self.num_layers - 1:
             self.advance(incoming)
 

@@ -115,6 +115,9 @@ def test_cache_class():
         cache.update_kv_cache(rows, rows, 0)
     assert cache.lengths.sum() == 0 and cache.get_kv_len() == 100  # (refused before anything changed)
     cache.clear()
+    with pytest.raises(ValueError):
+        cache.update_kv_cache(rows, rows, 0)  # (host tensors)
+    assert cache.lengths.sum() == 0 and cache.incoming == 0 and cache.get_kv_len() == 0
     with pytest.raises(ValueError, match="in a step of"):
         cache.update_kv_cache(rows, rows, 1)
     with pytest.raises(ValueError, match="in a step of"):
