@@ -595,6 +595,35 @@ def test_captured_steps_follow_the_device(gpu):
             pos.add_(T)
 
 
+def test_captured_prompt_pieces(gpu):
+    """Many rows captured with their shares of a long cache by three graphs that are replayed in turn, with
+    eager calls between: lengths and counts are read at each replay."""
+    _say("kv8 captured pieces")
+    g = torch.Generator().manual_seed(14)
+    caches = _filled(2, 2, 5000, 64, g, gpu)
+    lengths = torch.tensor([100, 5000], dtype=torch.int32, device=gpu)
+    counts = torch.tensor([40, 40], dtype=torch.int32, device=gpu)
+    runs = []
+    for T, window in ((40, None), (13, 2800), (3, None)):
+        q = _queries(2, 8, T, g, gpu)
+        call = lambda q=q, window=window: shadowkv.kv8_attn(q, *caches, lengths, counts, block=64,  # noqa: E731
+                                                            window=window)
+        call()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with capture_graph(graph, gpu):
+            out = call()
+        runs.append((graph, out, q, window, call))
+    for L, n in (([5000, 37], [40, 2]), ([0, 4999], [1, 13]), ([3000, 2999], [0, 40]), ([5000, 5000], [13, 40])):
+        lengths.copy_(torch.tensor(L, dtype=torch.int32))
+        counts.copy_(torch.tensor(n, dtype=torch.int32))
+        for graph, out, q, window, call in runs:
+            graph.replay()
+            got = out.clone()
+            assert torch.equal(got, call())
+            _check_attn(q, caches, L, n, 64, window, got=got)
+
+
 def test_other_stream_and_repeats(gpu):
     """Calls on another stream than the default one, two at once, the same call twice: the same bits."""
     _say("kv8 streams")
