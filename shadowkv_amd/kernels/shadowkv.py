@@ -1182,7 +1182,7 @@ KV8_MAX_TOKENS = 2 ** 30
 
 
 def _no_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+    if torch.is_grad_enabled() and any([t.requires_grad for t in tensors]):
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
@@ -1246,7 +1246,10 @@ def _kv8_pair(k8, v8, k_scale, v_scale, block):
     if index < 0 or v8.get_device() != index or k_scale.get_device() != index or v_scale.get_device() != index:
         raise ValueError("k8, v8 and their scales must be on one device")
     geo = _kv8_cache(k8, k_scale, "k8", block)
-    if geo != _kv8_cache(v8, v_scale, "v8", block):
+    alike = (v8.dtype is k8.dtype and v8.shape == k8.shape and v8.stride() == k8.stride() and not v8.data_ptr() & 15
+             and v_scale.dtype is k_scale.dtype and v_scale.shape == k_scale.shape
+             and v_scale.stride() == k_scale.stride())
+    if not alike and geo != _kv8_cache(v8, v_scale, "v8", block):
         raise ValueError("k8 and v8 (and their scales) must share a layout")
     return *geo, index
 
