@@ -150,8 +150,8 @@ __device__ __forceinline__ float sum_of_rows(float x) {
 // v_mfma_f32_16x16x32_bf16 (a row of the queries a column) leaves a lane with 8 keys' scores of one row, which is the
 // second operand of O^T = V^T P^T, whose first is the lane's 8 tokens of one dim: neither probabilities nor
 // values cross lanes. Measured (MI355X, 4 query heads on each of 8 kv heads): 8 sequences of 122880 tokens 306 us, 6.6
-// TB/s; 24 windows of 8192 keys and 64 sinks 74 us, 5.3 TB/s; 5 tokens each of 4 sequences of up to 30011 42 us, 3.7
-// TB/s (two tiles of rows leave two waves a SIMD, and the conversions and exponentials 20 us of it).
+// TB/s; 24 windows of 8192 keys and 64 sinks 74 us, 5.3 TB/s; 5 tokens each of 4 sequences of up to 30011 40 us, 3.9
+// TB/s (two tiles of rows leave two waves a SIMD to hide the loads' latency).
 constexpr int kGroup = 32;
 constexpr int kGroupShift = 5;
 constexpr int kMinGroups = 8;   // a chunk's groups of 32 keys, at least
@@ -259,17 +259,20 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
   u32x4 kr[2][2];
   u32x2 vr[8];
   float kc[2], vc[2];
-  auto load = [&](int i) __attribute__((always_inline)) {
+  auto load_keys = [&](int i, u32x4 (&k)[2][2], float (&c)[2]) __attribute__((always_inline)) {
     const int j0 = seen.at(i) * kGroup;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       const uint8_t* row = kh + static_cast<int64_t>(min(j0 + 16 * u + li, pmax)) * a.c_ss;
-      kr[u][0] = *reinterpret_cast<const u32x4*>(row);
-      kr[u][1] = *reinterpret_cast<const u32x4*>(row + 64);
-      const int blk = min(j0 + 16 * u, pmax) >> a.block_shift;
-      kc[u] = ksh[blk];
-      vc[u] = vsh[blk];
+      k[u][0] = *reinterpret_cast<const u32x4*>(row);
+      k[u][1] = *reinterpret_cast<const u32x4*>(row + 64);
+      c[u] = ksh[min(j0 + 16 * u, pmax) >> a.block_shift];
     }
+  };
+  auto load_values = [&](int i) __attribute__((always_inline)) {
+    const int j0 = seen.at(i) * kGroup;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) vc[u] = vsh[min(j0 + 16 * u, pmax) >> a.block_shift];
     // (values, whole rows of each line a load, with the streaming hint: 8 sequences of 122880 tokens 340 -> 317 us;
     // keys, half of a line a load, gain nothing from it)
 #pragma unroll
@@ -280,8 +283,23 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
             vh + static_cast<int64_t>(min(j0 + 16 * u + 4 * grp + r, pmax)) * a.c_ss));
   };
 
+  // With two tiles of rows there are but two waves a SIMD, and registers for the next group's keys (5 drafted tokens of
+  // 4 sequences: 43 -> 41 us; its values too: 44).
+  constexpr bool kAhead = kTiles == 2;
+  u32x4 kn[2][2];
+  float kcn[2];
+  if (kAhead && i0 + wave < i1) load_keys(i0 + wave, kn, kcn);
   for (int i = i0 + wave; i < i1; i += kWaves) {
-    load(i);
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        kr[u][0] = kn[u][0];
+        kr[u][1] = kn[u][1];
+        kc[u] = kcn[u];
+      }
+    } else load_keys(i, kr, kc);
+    load_values(i);
+    if (kAhead) load_keys(min(i + kWaves, i1 - 1), kn, kcn);
     const int j0 = seen.at(i) * kGroup;
     f32x4 s[kTiles][2];
 #pragma unroll
