@@ -541,11 +541,10 @@ __global__ void __launch_bounds__(256) few_join_kernel(Args a) {
 // wave, a row a lane, and walks the tiles of 64 keys that any of them sees, or a share of them where there are too few
 // rows to fill the chip. Keys and values are read once a tile, turned into 16 bits (the values transposed) by the
 // threads that read them, and shared through LDS, the next tile on its way meanwhile. Measured (MI355X): 8192 causal
-// tokens of 32 heads over 8, 540 us, 1.02 PFLOP/s where a large bf16 GEMM has 1.22; 2048 tokens behind up to 31285
-// others, 16 heads on each of 2 kv heads, a window of 8192, two sequences, 520 us, 0.93 PFLOP/s. Of a tile's time,
-// the matrix instructions of a wave take 1024 cycles, as many as the four SIMDs' reads of their operands take of LDS,
-// and the vector work (conversions, exponentials, maximum) 870, which hides behind the former only in part; the clock
-// is at 1.9 of 2.4 GHz under this load.
+// tokens of 32 heads over 8, 533 us, 1.03 PFLOP/s where a large bf16 GEMM has 1.22; 2048 tokens behind up to 31285
+// others, 16 heads on each of 2 kv heads, a window of 8192, two sequences, 515 us, 0.94 PFLOP/s. Counters (the prompt):
+// the matrix cores are busy in 46% of the cycles, the vector units in 47%, LDS in 32%, at a clock of 1.9 of 2.4 GHz:
+// the power is the limit, and vector work that hides behind the matrix instructions only in part.
 constexpr int kTile = 64;
 constexpr int kTileShift = 6;
 constexpr int kRowsWave = 32;
@@ -892,6 +891,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
           o[j & 3] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f[j & 3]),
                                                             __builtin_bit_cast(f16x8, part[(j - 16) >> 2]), o[j & 3], 0,
                                                             0, 0);
+        asm volatile("s_nop 0");  // (a slot for the SIMD's other wave: 544 -> 540 us; two: 545)
         // (vector work, evenly: the maximum and the reference, 16 pairs of probabilities, each before the product that
         // takes it, and between those the tiles on their way)
         constexpr int kPair[32] = {-1, -1, -1, -1, 0, 1, -1, 2, 3, -1, 4, 5, -1, 6, 7, -1,
