@@ -8,7 +8,7 @@
 //
 // Bound: HBM bytes (written rows 2 + 1 per element, read rows 1 + 2); a decoded token is a launch. Measured (MI355X, 8
 // heads): 122880 tokens written in 140 us, 5.4 TB/s (a large copy has 4.7); 100003 rows read in 63, 4.9 TB/s; a
-// token of each of 8 sequences written in 4.4 on the device (12.1 a call from Python).
+// token of each of 8 sequences written in 4.4 on the device (10.8 a call from Python).
 #include "skv_common.h"
 
 namespace {

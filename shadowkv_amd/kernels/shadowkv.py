@@ -1178,7 +1178,8 @@ def gather_copy_misses_to_slots(values, v_cache_buffer, miss_ids, cnts, miss_slo
 KV8_BLOCKS = (16, 32, 64, 128)
 KV8_MAX_TOKENS = 2 ** 30
 
-# These checks stand in front of calls of a few microseconds: the usual layouts pass on few attribute reads.
+# These checks stand in front of calls of a few microseconds: a layout is looked at once, the usual ones pass on few
+# attribute reads.
 
 
 def _no_grad(what: str, *tensors) -> None:
@@ -1186,9 +1187,9 @@ def _no_grad(what: str, *tensors) -> None:
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 
-def _strides(t: torch.Tensor, n: int) -> tuple:
-    """The first n strides of t, those of axes with one entry as 0 (torch leaves them open)."""
-    return tuple(st if sz > 1 else 0 for st, sz in zip(t.stride()[:n], t.shape))
+def _strides(shape, strides, n: int) -> tuple:
+    """The first n strides, those of axes with one entry as 0 (torch leaves them open)."""
+    return tuple([st if sz > 1 else 0 for st, sz in zip(strides[:n], shape)])
 
 
 def _rows128(t: torch.Tensor, name: str):
@@ -1201,69 +1202,71 @@ def _rows128(t: torch.Tensor, name: str):
     sb, sh, st, se = t.stride()
     if se == 1 and not (sb | sh | st) & 7 and not t.data_ptr() & 15:
         return t, (sb, sh, st)
-    strides = _strides(t, 3)
+    strides = _strides(shape, t.stride(), 3)
     if se != 1 or t.data_ptr() & 15 or any(s % 8 for s in strides):
         t = t.clone(memory_format=torch.contiguous_format)
-        strides = _strides(t, 3)
+        strides = _strides(shape, t.stride(), 3)
     return t, strides
 
 
 def _kv8_ints(t: torch.Tensor, name: str, B: int, index: int) -> int:
-    _dev(t, name, torch.int32)
-    if t.dim() != 1 or t.shape[0] != B or not t.is_contiguous() or t.get_device() != index:
-        raise ValueError(f"{name} must be {B} contiguous int32 on the caches' device, got {tuple(t.shape)} on {t.device}")
+    if t.dtype is not torch.int32 or t.get_device() != index or t.shape != (B,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be {B} contiguous int32 on the caches' device, got {tuple(t.shape)} {t.dtype} "
+                         f"on {t.device}")
     return t.data_ptr()
 
 
-def _kv8_cache(codes: torch.Tensor, scale: torch.Tensor, name: str, block: int):
-    """Checks one cache but for where its codes are; returns ((B, H, cap), strides of the codes, of the scales)."""
-    if block not in KV8_BLOCKS:
-        raise ValueError(f"block={block} must be one of {KV8_BLOCKS}")
-    _dev(scale, f"{name} scale", torch.float32)
-    if codes.dtype != torch.float8_e4m3fn:
-        raise ValueError(f"{name} must be torch.float8_e4m3fn, got {codes.dtype}")
-    shape = codes.shape
-    if len(shape) != 4 or shape[3] != 128 or 0 in shape or codes.stride(3) != 1 or codes.data_ptr() & 15:
-        raise ValueError(f"{name} {tuple(shape)} must be [B, H, capacity, 128] with contiguous rows, 16-byte aligned")
-    B, H, cap, _ = shape
-    if cap > KV8_MAX_TOKENS:
-        raise ValueError(f"{name} holds {cap} tokens (at most {KV8_MAX_TOKENS})")
-    if codes.is_contiguous():
-        strides = (H * cap * 128, cap * 128, 128)
-    else:
-        strides = _strides(codes, 3)
-        if any(s % 16 for s in strides):
-            raise ValueError(f"{name}: strides {strides} must be multiples of 16")
-    sshape, blocks = scale.shape, (cap + block - 1) // block
-    if len(sshape) != 3 or sshape[0] != B or sshape[1] != H or sshape[2] < blocks or scale.stride(2) != 1:
-        raise ValueError(f"{name} scale {tuple(sshape)} must be [{B}, {H}, {blocks} or more] with contiguous rows")
-    return (B, H, cap), strides, (H * sshape[2], sshape[2]) if scale.is_contiguous() else _strides(scale, 2)
-
-
-def _kv8_pair(k8, v8, k_scale, v_scale, block):
-    """Checks keys and values of one layout; returns ((B, H, cap), strides of codes, of scales, device index)."""
-    index = k8.get_device()
-    if index < 0 or v8.get_device() != index or k_scale.get_device() != index or v_scale.get_device() != index:
-        raise ValueError("k8, v8 and their scales must be on one device")
-    geo = _kv8_cache(k8, k_scale, "k8", block)
-    alike = (v8.dtype is k8.dtype and v8.shape == k8.shape and v8.stride() == k8.stride() and not v8.data_ptr() & 15
-             and v_scale.dtype is k_scale.dtype and v_scale.shape == k_scale.shape
-             and v_scale.stride() == k_scale.stride())
-    if not alike and geo != _kv8_cache(v8, v_scale, "v8", block):
-        raise ValueError("k8 and v8 (and their scales) must share a layout")
-    return *geo, index
-
-
-def _distinct(t: torch.Tensor) -> bool:
-    """Whether no two elements of t can share memory."""
-    if t.is_contiguous():
-        return True
+def _distinct(shape, strides) -> bool:
+    """Whether no two elements of such a tensor can share memory."""
     extent = 1
-    for stride, size in sorted((st, sz) for st, sz in zip(t.stride(), t.shape) if sz > 1):
+    for stride, size in sorted([(st, sz) for st, sz in zip(strides, shape) if sz > 1]):
         if stride < extent:
             return False
         extent += (size - 1) * stride
     return True
+
+
+@functools.lru_cache(maxsize=256)
+def _kv8_layout(name: str, block: int, shape, strides, dtype, s_shape, s_strides, s_dtype):
+    """Checks the layout of a cache and its scales; returns ((B, H, cap), strides of the codes, of the scales, whether
+    no two elements share memory)."""
+    if block not in KV8_BLOCKS:
+        raise ValueError(f"block={block} must be one of {KV8_BLOCKS}")
+    if dtype != torch.float8_e4m3fn or s_dtype != torch.float32:
+        raise ValueError(f"{name} must be torch.float8_e4m3fn with float32 scales, got {dtype} and {s_dtype}")
+    if len(shape) != 4 or shape[3] != 128 or 0 in shape or strides[3] != 1:
+        raise ValueError(f"{name} {tuple(shape)} must be [B, H, capacity, 128] with contiguous rows")
+    B, H, cap, _ = shape
+    if cap > KV8_MAX_TOKENS:
+        raise ValueError(f"{name} holds {cap} tokens (at most {KV8_MAX_TOKENS})")
+    c_strides, blocks = _strides(shape, strides, 3), (cap + block - 1) // block
+    if any(st % 16 for st in c_strides):
+        raise ValueError(f"{name}: strides {c_strides} must be multiples of 16")
+    if len(s_shape) != 3 or s_shape[0] != B or s_shape[1] != H or s_shape[2] < blocks or \
+            (s_shape[2] > 1 and s_strides[2] != 1):
+        raise ValueError(f"{name} scale {tuple(s_shape)} must be [{B}, {H}, {blocks} or more] with contiguous rows")
+    return ((B, H, cap), c_strides, _strides(s_shape, s_strides, 2),
+            _distinct(shape, strides) and _distinct(s_shape, s_strides))
+
+
+def _kv8_cache(codes: torch.Tensor, scale: torch.Tensor, name: str, block: int):
+    """_kv8_layout of one cache, and that its codes are 16-byte aligned."""
+    layout = _kv8_layout(name, block, codes.shape, codes.stride(), codes.dtype, scale.shape, scale.stride(),
+                         scale.dtype)
+    if codes.data_ptr() & 15:
+        raise ValueError(f"{name} must be 16-byte aligned")
+    return layout
+
+
+def _kv8_pair(k8, v8, k_scale, v_scale, block):
+    """Checks keys and values of one layout; returns it and the device index."""
+    index = k8.get_device()
+    if index < 0 or v8.get_device() != index or k_scale.get_device() != index or v_scale.get_device() != index:
+        raise ValueError("k8, v8 and their scales must be on one device")
+    layout = _kv8_cache(k8, k_scale, "k8", block)
+    if layout != _kv8_cache(v8, v_scale, "v8", block):
+        raise ValueError("k8 and v8 (and their scales) must share a layout")
+    return *layout, index
 
 
 def _call_on(index: int, name: str, *args) -> None:
@@ -1283,7 +1286,7 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
     A block's scale is the smallest power of two under which its new rows fit; where it holds older rows (before
     start[b]) it never falls, and they are encoded again where it grows. Infinities become NaN. Nothing else in
     the caches changes."""
-    (B, H, cap), c_strides, s_strides, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    (B, H, cap), c_strides, s_strides, distinct, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
     _no_grad("kv8_write", k, v)
     k, k_strides = _rows128(k, "k")
     v, v_strides = _rows128(v, "v")
@@ -1291,8 +1294,7 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
         raise ValueError(f"kv8_write: k {tuple(k.shape)} v {tuple(v.shape)} for caches of [{B}, {H}]")
     if k.get_device() != index or v.get_device() != index:
         raise ValueError("kv8_write: rows and caches must be on one device")
-    if not (_distinct(k8) and _distinct(v8) and _distinct(k_scale) and _distinct(v_scale)) or \
-            k8.data_ptr() == v8.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
+    if not distinct or k8.data_ptr() == v8.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
         raise ValueError("kv8_write: the caches must not share memory with themselves or each other")
     sp = _kv8_ints(start, "start", B, index)
     cp = None if counts is None else _kv8_ints(counts, "counts", B, index)
@@ -1301,10 +1303,10 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
 
 
 def _kv8_read(codes, scale, chunk_ids, chunk_size, start, rows, block):
-    (B, H, cap), c_strides, s_strides = _kv8_cache(codes, scale, "codes", block)
+    (B, H, cap), c_strides, s_strides, _ = _kv8_cache(codes, scale, "codes", block)
     index = scale.get_device()
-    if codes.is_cuda and codes.get_device() != index:
-        raise ValueError("the codes and their scales must be on one device")
+    if index < 0 or (codes.is_cuda and codes.get_device() != index):
+        raise ValueError("the scales must be on a device, and codes that are on one beside them")
     out = torch.empty(B, H, rows, 128, dtype=torch.bfloat16, device=scale.device)
     _call_on(index, "skv_kv8_read", device_address(codes), *c_strides, scale.data_ptr(), *s_strides,
              None if chunk_ids is None else chunk_ids.data_ptr(), chunk_size, start, out.data_ptr(), B, H, rows, cap,
@@ -1346,7 +1348,7 @@ def kv8_attn(q, k8, v8, k_scale, v_scale, lengths, counts=None, *, block=64, sca
     sequence. lengths (tokens held, the new ones among them; clamped to [0, capacity]), counts: device int32 [B],
     read when the kernels run. Queries that see nothing and those past counts[b] give zeros. What a query does
     not see may hold anything, NaN too, in the codes and in their scales. scale: 1 / sqrt(128) by default."""
-    (B, H, cap), c_strides, s_strides, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    (B, H, cap), c_strides, s_strides, _, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
     _no_grad("kv8_attn", q)
     q, q_strides = _rows128(q, "q")
     Bq, Hq, T, _ = q.shape
