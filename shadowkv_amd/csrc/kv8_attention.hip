@@ -594,8 +594,12 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int i = blockIdx.x;
   const int BH = a.B * a.H;
-  const int bh = i % BH;
+  int bh = i % BH;
   i /= BH;
+  // Consecutive workgroups go to the XCDs in turn: one (sequence, kv head) stays with its XCDs, whose L2 holds its
+  // keys, while the chip takes on one set of workgroups; for the next set the sequences, whose work differs, change
+  // places (four of 2000 to 8000 tokens: 458 -> 408 us; at every tile 387, but two windowed pieces 512 -> 531).
+  bh = (bh / a.H + static_cast<int>(static_cast<int64_t>(i) * BH / (2048 / kWaves))) % a.B * a.H + bh % a.H;
   const int split = i % a.splits;
   const int rt = a.rtiles - 1 - i / a.splits;  // the longest first
   const int b = bh / a.H, h = bh - b * a.H;
@@ -1150,10 +1154,12 @@ struct Plan {
   int64_t parts;  // partial rows of 128 + 2 floats
 };
 
-// Tiles of 64 keys from which workgroups of 8 waves take the rows, if more than 128: a thread then turns half as many
-// codes into 16 bits, but a tile's barrier holds a whole CU (MI355X, us, 4 query heads on each of 8 kv heads, 4 waves /
-// 8: 2000 tokens of a prompt 38 / 45, 4096 110 / 105, 16384 1389 / 1365; 24 sequences' 64 tokens on 1000 keys 31.7 /
-// 31.2, on 4000 86 / 80, on 16000 334 / 311; with up to 128 rows the added waves have none: 9 tokens 50 / 56).
+// Tiles of 64 keys from which workgroups of 8 waves take the rows, if more than 128 and enough for every CU: a thread
+// then turns half as many codes into 16 bits, but a tile's barrier holds a whole CU, and a CU without a second
+// workgroup waits for the longest (MI355X, us, 4 waves / 8: 4 query heads on each of 8 kv heads, 2000 tokens of a
+// prompt 38 / 45, 4096 110 / 105, 16384 1389 / 1365, 4 sequences' 100 tokens on 30000 keys 171 / 160; three ragged
+// prompts of 4000 on 4 heads, 192 workgroups of 8, 90 / 110; with up to 128 rows the added waves have none: 9 tokens
+// 50 / 56).
 constexpr int kLongTiles = 40;
 
 // Shares of a row tile's keys, of at least 4 tiles, where the workgroups alone would leave part of the chip idle: as
@@ -1189,11 +1195,14 @@ Plan plan_of(int B, int H, int G, int T, int cap, int window, int sinks) {
     return p;
   }
   const int64_t tiles = (keys + kTile - 1) / kTile;
-  p.waves = R > 4 * kRowsWave && tiles >= kLongTiles ? 8 : 4;
-  const int tile = p.waves * kRowsWave;
-  p.rtiles = static_cast<int>((R + tile - 1) / tile);
-  const int64_t wgs = static_cast<int64_t>(B) * H * p.rtiles;
-  p.splits = shares(tiles, wgs, 2048 / p.waves, static_cast<double>(B) * H * R);
+  int64_t wgs = 0;
+  for (p.waves = R > 4 * kRowsWave && tiles >= kLongTiles ? 8 : 4;; p.waves = 4) {
+    const int64_t tile = p.waves * kRowsWave, resident = 2048 / p.waves;  // workgroups at once on the chip's 256 CUs
+    p.rtiles = static_cast<int>((R + tile - 1) / tile);
+    wgs = static_cast<int64_t>(B) * H * p.rtiles;
+    p.splits = shares(tiles, wgs, resident, static_cast<double>(B) * H * R);
+    if (p.waves == 4 || wgs * p.splits >= resident) break;
+  }
   p.grid = wgs * p.splits;
   p.parts = p.splits > 1 ? static_cast<int64_t>(B) * H * R * p.splits : 0;
   return p;

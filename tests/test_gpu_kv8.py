@@ -521,6 +521,38 @@ def test_attn_many_on_long_caches_odd(gpu, window, sinks):
         assert torch.equal(got[b].isnan().any(-1), hit.unsqueeze(1).expand(50, 8))
 
 
+@pytest.mark.parametrize("window,sinks", [(None, 0), (6800, 0), (6790, 70)])
+def test_attn_many_rows_of_many_heads(gpu, window, sinks):
+    """Enough workgroups of more than 128 rows, over shares of a long cache, for every CU (they are then larger): ends
+    of windows, waves with no rows, padding, NaN seen by some, scales of any size, hidden ones of NaN."""
+    _say(f"kv8_attn many rows and heads window={window}")
+    g = torch.Generator().manual_seed(17)
+    B, H, G, T, cap, block = 2, 8, 4, 33, 8000, 16
+    q = _queries(B, H * G, T, g, gpu)
+    caches = _filled(B, H, cap, block, g, gpu)
+    _check_attn(q, caches, [8000, 4811], None, block, window, sinks)
+    _check_attn(q, caches, [7933, 20], [T, 7], block, window, sinks)
+    _check_attn(q, caches, [7001, 0], [1, T], block, window, sinks)
+    v8 = caches[1].view(torch.uint8)
+    v8[0, 0, 7975, 5] = v8[0, 1, 1190, 9] = v8[0, 2, 3, 127] = v8[0, 3, 5000, 64] = 0x7f
+    v8[1, 0, 7980:7990, 64:70] = 0xff
+    _check_attn(q, caches, [8000, 7999], None, block, window, sinks)
+    caches = _filled(B, H, cap, block, g, gpu)
+    caches[3].mul_(torch.exp2(torch.randint(-9, 9, caches[3].shape, generator=g).float()).to(gpu))
+    caches[2].mul_((0.6 + torch.rand(caches[2].shape, generator=g)).to(gpu))
+    _check_attn(q, caches, [8000, 7977], None, block, window, sinks)
+    lengths = [8000, 7990]
+    caches[2][:, :, 7975 // block] = math.nan  # seen by the last queries only
+    caches[3][:, :, 1185 // block] = math.nan  # with a window, by the first ones only
+    got = shadowkv.kv8_attn(q, *caches, torch.tensor(lengths, dtype=torch.int32, device=gpu), block=block,
+                            window=window, sinks=sinks).cpu()
+    for b, L in enumerate(lengths):
+        j = torch.arange(L) // block
+        hit = _see(T, T, L, window, sinks)[:, (j == 7975 // block) | (j == 1185 // block)].any(1)
+        assert torch.equal(got[b].isnan().all(-1), hit.unsqueeze(1).expand(T, H * G))
+        assert torch.equal(got[b].isnan().any(-1), hit.unsqueeze(1).expand(T, H * G))
+
+
 def test_attn_long_and_uneven(gpu):
     """A batch of one long and many short sequences (chunks of several groups to a wave, 70 sequences over two
     passes of the plan), and a few tokens of long ones (keys split over workgroups)."""
