@@ -681,12 +681,16 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
 #pragma unroll
     for (int c = 0; c < kKeyLoads; ++c) kheld[c] = __builtin_amdgcn_raw_buffer_load_b128(src, x.kmine, 16 * c, 0);
   };
-  auto fetch_values = [&](const Lane& x, __amdgpu_buffer_rsrc_t src) __attribute__((always_inline)) {
+  // (a buffer's bounds are checked against the vector offset alone: a row's place in its group goes there wherever the
+  // sequence may end inside the tile)
+  auto fetch_values = [&](auto whole, const Lane& x, __amdgpu_buffer_rsrc_t src) __attribute__((always_inline)) {
+    constexpr bool kCut = !decltype(whole)::value;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       const int at = ((e & 3) + 8 * (e >> 2)) * stride;
-      if constexpr (kWaves == 4) vheld[e] = __builtin_amdgcn_raw_buffer_load_b32(src, x.vmine, at, 0);
-      else vheld[e] = __builtin_amdgcn_raw_buffer_load_b16(src, x.vmine, at, 0);
+      const int vector = kCut ? x.vmine + at : x.vmine, scalar = kCut ? 0 : at;
+      if constexpr (kWaves == 4) vheld[e] = __builtin_amdgcn_raw_buffer_load_b32(src, vector, scalar, 0);
+      else vheld[e] = __builtin_amdgcn_raw_buffer_load_b16(src, vector, scalar, 0);
     }
   };
   auto place_chunk = [&](const Lane& x, int buf, int c) __attribute__((always_inline)) {
@@ -907,13 +911,13 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
         else if (j == 18) fetch_keys(g, whole_rows(kh, i + 3));
         else if (j == 21 || j == 24) place_pairs(g, par ^ 1, j / 3 - 7, factor, x);
         else if ((j == 27 || j == 28) && kValueDims == 4) place_pairs(g, par ^ 1, j - 25, factor, x);
-        else if (j == 29) fetch_values(g, whole_rows(vh, i + 2));
+        else if (j == 29) fetch_values(std::true_type{}, g, whole_rows(vh, i + 2));
         else if (j == 30) next_factors(i);
         __builtin_amdgcn_sched_barrier(0);
       }
     };
     fetch_keys(g, whole_rows(kh, from));
-    fetch_values(g, whole_rows(vh, from));
+    fetch_values(std::true_type{}, g, whole_rows(vh, from));
     place_keys(g, 0);
     place_f16(g, from, 0);
     __builtin_amdgcn_sched_barrier(0);
@@ -921,7 +925,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
     place_keys(g, 1);
     __builtin_amdgcn_sched_barrier(0);
     fetch_keys(g, whole_rows(kh, from + 2));
-    fetch_values(g, whole_rows(vh, from + 1));
+    fetch_values(std::true_type{}, g, whole_rows(vh, from + 1));
     __syncthreads();
     factors[0] = factors_of(fetch_scales(from));
     factors[1] = factors_of(fetch_scales(from + 1));
@@ -937,7 +941,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
 #pragma unroll
         for (int y = 0; y < kValueDims; ++y) place_pairs(g, par ^ 1, y, factor, x);
         fetch_keys(g, whole_rows(kh, i + 3));
-        fetch_values(g, whole_rows(vh, i + 2));
+        fetch_values(std::true_type{}, g, whole_rows(vh, i + 2));
         next_factors(i);
       }
       return;
@@ -989,7 +993,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
     const int p = mine.query ? p0 + mine.t : pmax;
     __syncthreads();  // every wave is past the tiles before these
     fetch_keys(g, tile_rows(kh, seen.at(from)));
-    fetch_values(g, tile_rows(vh, seen.at(from)));
+    fetch_values(std::false_type{}, g, tile_rows(vh, seen.at(from)));
     for (int i = from; i < to; ++i) {
       const int buf = (i - from) & 1, tile = seen.at(i);
       place_keys(g, buf);
@@ -998,7 +1002,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
       __syncthreads();  // (and every wave is past the tile before last, whose place the next one takes)
       if (i + 1 < to) {
         fetch_keys(g, tile_rows(kh, seen.at(i + 1)));
-        fetch_values(g, tile_rows(vh, seen.at(i + 1)));
+        fetch_values(std::false_type{}, g, tile_rows(vh, seen.at(i + 1)));
       }
       if (idle) continue;  // wave-uniform
       f32x16 s[2];
