@@ -228,14 +228,15 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
   const int li = lane & 15, grp = lane >> 4;
 
   // Q as the B operand: lane (li, grp) holds row li of a tile, in step s dims 64 (s / 2) + 16 grp + 8 (s % 2) and on.
-  // Rows past the last, and of padding, ride along with the last query, and give nothing in the end.
+  // Rows past the last, and of padding, ride along with the last query (padding's own memory, which may hold anything, is
+  // not read), and give nothing in the end.
   bf16x8 qf[kTiles][4];
   int p[kTiles];
 #pragma unroll
   for (int y = 0; y < kTiles; ++y) {
     const int row = min(16 * y + li, R - 1), t = row / G;
     p[y] = t < n ? pmin + t : pmax;
-    const uint16_t* q = a.q + b * a.q_sb + (h * G + row - t * G) * a.q_sh + t * a.q_st + 16 * grp;
+    const uint16_t* q = a.q + b * a.q_sb + (h * G + row - t * G) * a.q_sh + min(t, max(n - 1, 0)) * a.q_st + 16 * grp;
 #pragma unroll
     for (int s = 0; s < 4; ++s)
       qf[y][s] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const u32x4*>(q + 64 * (s >> 1) + 8 * (s & 1)) ^
@@ -615,7 +616,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
   const int i0 = min(split * each, seen.total), i1 = min(i0 + each, seen.total);
 
   // Row li of the wave: query t, head g of the kv head's. Those past the last row, and of padding, ride along with the
-  // last query, and give nothing in the end.
+  // last query (padding's own memory, which may hold anything, is not read), and give nothing in the end.
   struct Row {
     int row, t, g;
     bool query;
@@ -633,7 +634,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
   u32x4 qf[8];
   {
     const Row x = row_of(threadIdx.x & 31);
-    const uint16_t* q = a.q + b * a.q_sb + (h * G + x.g) * a.q_sh + x.t * a.q_st + 8 * (lane >> 5);
+    const uint16_t* q = a.q + b * a.q_sb + (h * G + x.g) * a.q_sh + min(x.t, max(n - 1, 0)) * a.q_st + 8 * (lane >> 5);
 #pragma unroll
     for (int s = 0; s < 8; ++s) qf[s] = *reinterpret_cast<const u32x4*>(q + 16 * s);
     if (a.negative)
@@ -1124,7 +1125,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
   }
   const int64_t at = (static_cast<int64_t>(bh) * R + x.row) * a.splits + split;
   if (g.half == 0) {
-    a.ws_ml[2 * at] = m;
+    a.ws_ml[2 * at] = x.query ? m : -INFINITY;
     a.ws_ml[2 * at + 1] = l;
   }
   float* dst = a.ws_o + at * kD + 4 * g.half;
