@@ -60,3 +60,27 @@ def test_attn_padding_queries(gpu, H, G, T, cap):
                 torch.where(one > 0, -math.inf, -0.5), one * 3e38):
         x = torch.where(pad, torch.as_tensor(odd, device=gpu).to(BF16), q)
         assert torch.equal(call(x), want), odd
+
+
+@pytest.mark.parametrize("T,cap", [(1, 320), (6, 2500), (40, 320), (40, 2560), (300, 512)])
+def test_attn_scores_past_32_bits_steps(gpu, T, cap):
+    """Scores so large that neighbouring fp32 numbers differ by whole units, all equal: the mean of the values. Tolerance:
+    the output's rounding, 2^-8 of the value, the fp32 sums', 2^-23 a key; and a score S (in units of log2) that is a
+    product rounded to fp32 for one key and not for another moves a weight by up to 2^(2 S 2^-24), and the mean with it by
+    that much, less 1, of the values' range, but never out of their range."""
+    _say(f"kv8_attn large scores T={T} cap={cap}")
+    g = torch.Generator().manual_seed(T)
+    for size in (300.0, 3e4, 1.7e7, 3.1e9):
+        for factor in (0.11, 0.0937, 0.087):
+            k = torch.full((1, 2, cap, D), 13.0)
+            v = torch.rand(1, 2, cap, D, generator=g) + 1.0
+            caches = _caches(1, 2, cap, 32, g, gpu)
+            shadowkv.kv8_write(k.to(BF16).to(gpu), v.to(BF16).to(gpu), *caches, _ints([0], gpu), block=32)
+            vd = caches[1].cpu().double() * caches[3].cpu().double().repeat_interleave(32, 2)[:, :, :cap, None]
+            q = torch.full((1, 8, T, D), size).to(BF16).to(gpu)
+            got = shadowkv.kv8_attn(q, *caches, _ints([cap], gpu), block=32, scale=factor).cpu().double()
+            want = vd.cumsum(2)[:, :, cap - T:] / torch.arange(cap - T + 1, cap + 1).view(1, 1, T, 1)
+            want = want.repeat_interleave(4, 1).transpose(1, 2)
+            score = abs(q[0, 0, 0, 0].item()) * 13 * D * factor / math.log(2)
+            moved = min(1.0, math.expm1(min(1.0, 2 * score * 2.0 ** -24) * math.log(2))) * (vd.max() - vd.min())
+            assert ((got - want).abs() <= want * (2.0 ** -8 + cap * 2.0 ** -23) + moved).all(), (size, factor)
