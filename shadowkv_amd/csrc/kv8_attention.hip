@@ -4,7 +4,7 @@
 //   out[b, t, hq] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale q[b, hq, t] . k_j),  k_j = ks * code, v_j = vs * code
 //
 // over the keys j <= p of the query's position p = length_b - n_b + t, with a window w only those with j > p - w
-// or j < sinks. A query that sees nothing, or is padding (t >= n_b), gets zeros. Codes become bf16 (exactly) on
+// or j < sinks. A query that sees nothing (p < 0), or is padding (t >= n_b), gets zeros. Codes become bf16 (exactly) on
 // their way into the matrix cores; a key block's scale multiplies its scores and a value block's scale its
 // probabilities, so no dequantised row is ever formed. Scores, probabilities and sums are fp32. A probability
 // enters the product with the values as two bf16 parts (16 significant bits, an error of 2^-16 where the output's
@@ -456,7 +456,7 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
     __syncthreads();
     for (int i = threadIdx.x; i < rows * 32; i += 64 * kWaves) {
       const int g = i >> 5, d = 4 * (i & 31), row = 16 * y + g;
-      const bool query = row / G < n;  // (padding: as if it had seen nothing)
+      const bool query = row / G < n && pmin + row / G >= 0;  // (else padding, or it sees nothing: zeros)
       float top = m_lds[0][g];
 #pragma unroll
       for (int w = 1; w < kWaves; ++w) top = fmaxf(top, m_lds[w][g]);
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
         sum += f * *reinterpret_cast<const f32x4*>(&o_lds[w][g][d]);
       }
       if constexpr (kWhole) {
-        const float inv = query && lsum != 0.f ? 1.f / lsum : 0.f;  // (nothing seen: zeros)
+        const float inv = 1.f / lsum;
         const u32x2 out = {skv::f2bf2(sum[0] * inv, sum[1] * inv), skv::f2bf2(sum[2] * inv, sum[3] * inv)};
         const int t = row / G;
         const int64_t at = (static_cast<int64_t>(b) * a.T + t) * a.H * G + h * G + row - t * G;
@@ -486,10 +486,12 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
   }
 }
 
-// Joins n partial results (m, l, o), part i at index first + i * stride, into one row: 256 threads, 32 lanes of
-// four dims by 8 parts at a time. Every wave of it sees the same maximum and sum.
-__device__ __forceinline__ void join_parts(const float* ws_o, const float* ws_ml, int64_t first, int64_t stride, int n,
+// Joins n partial results (m, l, o), part i at index first + i * stride, into the row of sequence b's query t: 256
+// threads, 32 lanes of four dims by 8 parts at a time. Every wave of it sees the same maximum and sum.
+__device__ __forceinline__ void join_parts(const Args& a, int b, int t, int64_t first, int64_t stride, int n,
                                            uint16_t* out, f32x4 (&acc_lds)[8][32]) {
+  const float* ws_o = a.ws_o;
+  const float* ws_ml = a.ws_ml;
   const int lane = threadIdx.x & 63;
   float m = -INFINITY;
   for (int i = lane; i < n; i += 64) m = fmaxf(m, ws_ml[2 * (first + i * stride)]);
@@ -511,9 +513,11 @@ __device__ __forceinline__ void join_parts(const float* ws_o, const float* ws_ml
   if (threadIdx.x < 32) {
 #pragma unroll
     for (int i = 1; i < 8; ++i) acc += acc_lds[i][d];
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // (nothing seen: zeros)
-    *reinterpret_cast<u32x2*>(out + 4 * d) = {skv::f2bf2(acc[0] * inv, acc[1] * inv),
-                                              skv::f2bf2(acc[2] * inv, acc[3] * inv)};
+    const int count = count_of(a, b);
+    const bool query = t < count && length_of(a, b) - count + t >= 0;  // (else padding, or it sees nothing: zeros)
+    const float inv = 1.f / l;
+    const u32x2 row = {skv::f2bf2(acc[0] * inv, acc[1] * inv), skv::f2bf2(acc[2] * inv, acc[3] * inv)};
+    *reinterpret_cast<u32x2*>(out + 4 * d) = query ? row : u32x2{0u, 0u};
   }
 }
 
@@ -530,7 +534,7 @@ __global__ void __launch_bounds__(256) few_join_kernel(Args a) {
   }
   const int n = (few_groups(a, b).total + each - 1) / each;
   const int64_t R = static_cast<int64_t>(a.T) * a.G;
-  join_parts(a.ws_o, a.ws_ml, (static_cast<int64_t>(before) * a.H + h) * R + t * a.G + g, a.H * R, n,
+  join_parts(a, b, t, (static_cast<int64_t>(before) * a.H + h) * R + t * a.G + g, a.H * R, n,
              a.out + static_cast<int64_t>(blockIdx.x) * kD, acc_lds);
 }
 
@@ -1114,7 +1118,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
       o[d][r] = x.query ? v : 0.f;
     }
   if (a.splits == 1) {
-    const float inv = l == 0.f ? 0.f : 1.f / l;  // (nothing seen: zeros)
+    const float inv = x.query && p0 + x.t >= 0 ? 1.f / l : 0.f;  // (padding, or it sees nothing: zeros)
     uint16_t* dst = a.out + ((static_cast<int64_t>(b) * a.T + x.t) * a.H * G + h * G + x.g) * kD + 4 * g.half;
 #pragma unroll
     for (int d = 0; d < 4; ++d)
@@ -1142,7 +1146,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(Args a) {
   __shared__ f32x4 acc_lds[8][32];
   const int R = a.T * a.G, bh = blockIdx.x / R, row = blockIdx.x - bh * R;
   const int b = bh / a.H, h = bh - b * a.H, t = row / a.G, g = row - t * a.G;
-  join_parts(a.ws_o, a.ws_ml, static_cast<int64_t>(blockIdx.x) * a.splits, 1, a.splits,
+  join_parts(a, b, t, static_cast<int64_t>(blockIdx.x) * a.splits, 1, a.splits,
              a.out + ((static_cast<int64_t>(b) * a.T + t) * a.H * a.G + h * a.G + g) * kD, acc_lds);
 }
 

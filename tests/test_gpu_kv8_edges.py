@@ -84,3 +84,27 @@ def test_attn_scores_past_32_bits_steps(gpu, T, cap):
             score = abs(q[0, 0, 0, 0].item()) * 13 * D * factor / math.log(2)
             moved = min(1.0, math.expm1(min(1.0, 2 * score * 2.0 ** -24) * math.log(2))) * (vd.max() - vd.min())
             assert ((got - want).abs() <= want * (2.0 ** -8 + cap * 2.0 ** -23) + moved).all(), (size, factor)
+
+
+@pytest.mark.parametrize("T,cap", [(1, 320), (1, 2500), (6, 320), (6, 2500), (40, 320), (40, 2500)])
+def test_attn_scores_of_minus_infinity(gpu, T, cap):
+    """A query all of whose scores are -inf divides zero by zero, as by the formula: NaN. One that sees nothing is
+    zeros, and the others are what they are without it."""
+    _say(f"kv8_attn scores of -inf T={T} cap={cap}")
+    g = torch.Generator().manual_seed(T + cap)
+    caches = _filled(2, 2, cap, 32, g, gpu)
+    for c in caches[:2]:
+        c[..., 3] = torch.ones((), device=gpu).to(E4M3)
+    q = _queries(2, 8, T, g, gpu)
+    q[..., 3] = 0.0
+    at, n = _ints([256, T // 2], gpu), _ints([T, T], gpu)
+    want = shadowkv.kv8_attn(q, *caches, at, n, block=32)
+    assert not want.isnan().any() and (want[1, :T - T // 2] == 0).all()
+    x = q.clone()
+    x[:, 1::2, :, 3] = -math.inf
+    got = shadowkv.kv8_attn(x, *caches, at, n, block=32)
+    assert got[0, :, 1::2].isnan().all() and got[1, T - T // 2:, 1::2].isnan().all()
+    assert (got[1, :T - T // 2] == 0).all() and not got[:, :, ::2].isnan().any()
+    # (in 16 bits beside NaN, where the other call may have taken f16: 2^-11 of the values, and a bf16 rounding each)
+    assert (got[:, :, ::2].float() - want[:, :, ::2].float()).abs().max() <= want.float().abs().max() * 2.0 ** -7 + \
+        (caches[1].float().abs().amax() * caches[3].amax()) * 2.0 ** -10
