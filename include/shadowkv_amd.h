@@ -624,7 +624,8 @@ int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_stride_h, i
  * window > 0 only those with j > p - window or j < sinks:
  *   out[b, t, hq, :] = sum_j exp(scale q[b, hq, t] . k_j) v_j / sum_j exp(scale q[b, hq, t] . k_j)
  * over them, of kv head hq / (q_heads / kv_heads); zeros for a query that sees nothing (p < 0) and for t >= n_b.
- * Keys and values that a query does not see do not reach it, whatever they and their scales hold. Scores and sums in
+ * Keys and values that a query does not see do not reach it, whatever they and their scales hold; a seen block whose
+ * scale is NaN or infinite gives NaN. Scores and sums in
  * fp32; with more than 32 rows * q_heads / kv_heads and value scales that are powers of two within 2^12 of one another,
  * probabilities enter their product in f16, else (also beside NaN, or scores past 2^24) with 16 significant bits. out [batch, rows, q_heads, 128] bf16
  * (contiguous, 16-byte aligned). q: rows of 128 bf16 at q + b*q_stride_b + hq*q_stride_h + t*q_stride_t, multiples of

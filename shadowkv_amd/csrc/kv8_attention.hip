@@ -1037,7 +1037,14 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
 #pragma unroll
       for (int gk = 0; gk < 4; ++gk) {
         __builtin_amdgcn_sched_barrier(0);  // (one group's operands at a time: registers)
-        const float vsc = kF16 ? 1.f : scale_at(vsh, block_of(tile, gk));
+        float vsc = kF16 ? 1.f : scale_at(vsh, block_of(tile, gk));
+        if (!kF16 && !(__builtin_fabsf(vsc) < INFINITY)) {  // wave-uniform
+          // It reaches the rows that see a key of its block, whatever their probabilities, and no others.
+          bool some = false;
+          for (int e = 0; e < 8; ++e)
+            some |= sees(p, tile * kTile + 16 * gk + 4 * g.half + (e & 3) + 8 * (e >> 2), a.window, a.sinks);
+          vsc = some ? vsc : 0.f;
+        }
         u32x4 part[2];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
@@ -1050,8 +1057,7 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
           } else {
             l += x0 + x1;
             uint32_t first, second;
-            // (a hidden block's scale may be anything)
-            two_parts(x0 == 0.f ? 0.f : x0 * vsc, x1 == 0.f ? 0.f : x1 * vsc, first, second);
+            two_parts(x0 * vsc, x1 * vsc, first, second);
             part[0][e] = first;
             part[1][e] = second;
           }

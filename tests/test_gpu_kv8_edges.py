@@ -108,3 +108,30 @@ def test_attn_scores_of_minus_infinity(gpu, T, cap):
     # (in 16 bits beside NaN, where the other call may have taken f16: 2^-11 of the values, and a bf16 rounding each)
     assert (got[:, :, ::2].float() - want[:, :, ::2].float()).abs().max() <= want.float().abs().max() * 2.0 ** -7 + \
         (caches[1].float().abs().amax() * caches[3].amax()) * 2.0 ** -10
+
+
+@pytest.mark.parametrize("T,cap", [(1, 320), (1, 2500), (6, 320), (6, 2500), (50, 320), (50, 2500)])
+@pytest.mark.parametrize("odd", [math.nan, math.inf])
+def test_attn_seen_scales_that_are_not_finite(gpu, T, cap, odd):
+    """A value block of a NaN or infinite scale makes the rows that see a key of it NaN also where the key's probability
+    is too small for fp32 (zero times such a value), and no other rows."""
+    _say(f"kv8_attn seen scales T={T} cap={cap} {odd}")
+    g = torch.Generator().manual_seed(T)
+    at, block = [300, 256], 16
+    caches = _caches(2, 2, cap, block, g, gpu)
+    far = [1, 17, (300 - T // 2) // block]  # blocks of tiny probabilities; the last is seen by some of the rows only
+    k = torch.randn(2, 2, cap, D, generator=g)
+    for j in far:
+        k[:, :, j * block:(j + 1) * block] = -9.0
+    v = torch.randn(2, 2, cap, D, generator=g)
+    shadowkv.kv8_write(k.to(BF16).to(gpu), v.to(BF16).to(gpu), *caches, _ints([0, 0], gpu), block=block)
+    q = torch.full((2, 8, T, D), 4.0).to(BF16).to(gpu)
+    for window, sinks in ((None, 0), (40, 18)):
+        for j in far:
+            scales = caches[3].clone()
+            scales[:, :, j] = odd
+            got = shadowkv.kv8_attn(q, *caches[:3], scales, _ints(at, gpu), block=block, window=window, sinks=sinks).cpu()
+            for b, L in enumerate(at):
+                hit = _see(T, T, L, window, sinks)[:, torch.arange(L) // block == j].any(1)
+                assert torch.equal(got[b].isnan().all(-1), hit.unsqueeze(1).expand(T, 8)), (b, j, window)
+                assert torch.equal(got[b].isnan().any(-1), hit.unsqueeze(1).expand(T, 8)), (b, j, window)
