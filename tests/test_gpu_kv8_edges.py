@@ -135,3 +135,84 @@ def test_attn_seen_scales_that_are_not_finite(gpu, T, cap, odd):
                 hit = _see(T, T, L, window, sinks)[:, torch.arange(L) // block == j].any(1)
                 assert torch.equal(got[b].isnan().all(-1), hit.unsqueeze(1).expand(T, 8)), (b, j, window)
                 assert torch.equal(got[b].isnan().any(-1), hit.unsqueeze(1).expand(T, 8)), (b, j, window)
+
+
+def _check_sampled(q, caches, lengths, counts, block, window, sinks, rows):
+    """kv8_attn's rows t of `rows` against 64 bits. Tolerance, from the many-row form with probabilities p_j (at most
+    2^15, their largest at least 2^7) rounded to f16, p_j (1 + e_j) + z_j, |e_j| <= 2^-11, |z_j| <= 2^-25, over their own
+    sum: (sum of w_j |v_j - out| 2^-11 + keys 2^-32 2 top) (1 + 2^-9), w the softmax, top the largest value; beside it
+    twice a score's error (130 fp32 roundings of the sum of the products' magnitudes, 2^-22 for the exponential), the
+    fp32 sums (2^-24 a key, numerator and denominator) and a few last roundings (2^-21), each of top; and the output's
+    own rounding, 2^-8 of the value. (Two parts of bf16 are closer: 2^-15 of top would be left of the first term.)"""
+    got, again = [shadowkv.kv8_attn(q, *caches, _ints(lengths, q.device), _ints(counts, q.device), block=block,
+                                    window=window, sinks=sinks) for _ in range(2)]
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    got = got.cpu().double()
+    k8, v8, ks, vs = [c.cpu().double() for c in caches]
+    B, Hq, T, _ = q.shape
+    H, cap = k8.shape[1], k8.shape[2]
+    G, rows = Hq // H, torch.tensor(rows)
+    for b in range(B):
+        L, n = min(lengths[b], cap), T if counts is None else counts[b]
+        see = _see(n, T, L, window, sinks)[rows]
+        none = ~see.any(1)
+        assert (got[b, rows[none]] == 0).all()
+        assert (got[b, n:] == 0).all()
+        for h in range(H):
+            kk = k8[b, h, :L] * ks[b, h].repeat_interleave(block)[:L, None]
+            vv = v8[b, h, :L] * vs[b, h].repeat_interleave(block)[:L, None]
+            clean, top = vv.nan_to_num(0.0), vv.nan_to_num(0.0).abs().max()
+            for hq in range(h * G, (h + 1) * G):
+                x = q[b, hq].cpu().double()[rows] / math.sqrt(D)
+                w = torch.softmax((x @ kk.T).masked_fill(~see, -math.inf), -1).nan_to_num(0.0)
+                want = w @ clean
+                size = (x.abs() @ kk.abs().T).masked_fill(~see, 0.0).amax(1, keepdim=True)
+                away = torch.stack([w[i] @ (clean - want[i]).abs() for i in range(len(rows))])
+                tol = 2.0 ** -8 * want.abs() + 2.0 ** -11 * (1 + 2.0 ** -9) * away + top * (
+                    L * 2.0 ** -31 + 2 * (130 * 2.0 ** -24 * size + 2.0 ** -22) + 2 * L * 2.0 ** -24 + 2.0 ** -21)
+                nan = (see.double() @ vv.isnan().double()) > 0
+                g = got[b, rows, hq]
+                assert torch.equal(g.isnan(), nan), (b, hq)
+                err = (g - want).abs().masked_fill(nan, 0.0)
+                assert (err <= tol).all(), (b, hq, (err - tol).max(), err.max())
+
+
+@pytest.mark.parametrize("T,cap,window,sinks", [(1000, 3000, None, 0), (1000, 3000, 2600, 40), (750, 760, None, 0),
+                                                (750, 760, 200, 20)])
+def test_attn_many_rows_direct(gpu, T, cap, window, sinks):
+    """More workgroups than the chip holds at once, of 256 rows on long caches and of 128 on short ones, without shares
+    of the keys: sequences of different lengths and counts, windows, NaN seen by some rows, scales that f16 does not
+    hold together. Rows around the workgroups' and the waves' first and last."""
+    _say(f"kv8_attn many rows direct T={T} cap={cap} window={window}")
+    g = torch.Generator().manual_seed(T)
+    B, H, G, block = 3, 8, 4, 32
+    assert _lib.lib().skv_kv8_attn_workspace_bytes(B, H * G, H, T, cap, window or 0, sinks) == 0  # (no shares)
+    q = _queries(B, H * G, T, g, gpu)
+    caches = _filled(B, H, cap, block, g, gpu)
+    lengths, counts = [cap, cap - 211, T + 5], [T, T - 130, T]
+    rows = sorted({0, 1, 7, 8, 31, 32, 63, 64, 200, 333, 511, 512, T - 131, T - 130, T - 129, T - 64, T - 33, T - 2, T - 1})
+    _check_sampled(q, caches, lengths, counts, block, window, sinks, rows)
+    _check_sampled(q, caches, [T - 20, cap, 1], None, block, window, sinks, rows)
+    v8 = caches[1].view(torch.uint8)
+    for b, h, j, d in ((0, 0, cap - 40, 5), (0, 3, cap - T + 3, 127), (1, 7, lengths[1] - 300, 64), (2, 2, 9, 9)):
+        v8[b, h, j, d] = 0x7f
+    _check_sampled(q, caches, lengths, counts, block, window, sinks, rows)
+    caches = _filled(B, H, cap, block, g, gpu)
+    caches[3].mul_(torch.exp2(torch.randint(-9, 9, caches[3].shape, generator=g).float()).to(gpu))
+    _check_sampled(q, caches, lengths, counts, block, window, sinks, rows)
+
+
+@pytest.mark.parametrize("block", [16, 128])
+def test_read_rows_from_the_host(gpu, block):
+    """Rows of pinned host memory through kv8_read: the device cache's bits, from any first row, of other layouts too."""
+    _say(f"kv8_read from the host block={block}")
+    g = torch.Generator().manual_seed(block)
+    k8, _, ks, _ = _caches(2, 3, 333, block, g, gpu)
+    host = torch.empty(k8.shape, dtype=E4M3, pin_memory=True)
+    side = torch.empty(2, 333, 3, D, dtype=E4M3, pin_memory=True).permute(0, 2, 1, 3)
+    for c in (host, side):
+        c.view(torch.uint8).copy_(k8.view(torch.uint8))
+        for start, rows in ((0, 333), (17, 1), (100, 129), (332, 1)):
+            want = shadowkv.kv8_read(k8, ks, start, rows, block=block)
+            got = shadowkv.kv8_read(c, ks, start, rows, block=block)
+            assert torch.equal(got.view(torch.int16), want.view(torch.int16))
