@@ -603,7 +603,8 @@ int skv_linear_qkv_rope_append(const uint16_t* x, int64_t x_stride, const uint16
  * rows' largest finite magnitude is at most 448; the block's scale becomes need, or, where it holds older rows (of
  * its positions before start[b]), max(scale, need), and those are encoded again where that is larger.
  * Codes are value / scale to nearest even; infinities and NaN become NaN (the format has no infinity).
- * Every other code and scale stays as it is. The results do not depend on the order of execution. */
+ * Every other code and scale stays as it is. The results do not depend on the order of execution. The two caches'
+ * codes and scales share no memory with one another. */
 int skv_kv8_write(const uint16_t* k, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, const uint16_t* v,
                   int64_t v_stride_b, int64_t v_stride_h, int64_t v_stride_t, uint8_t* k8, uint8_t* v8,
                   int64_t c_stride_b, int64_t c_stride_h, int64_t c_stride_s, float* k_scale, float* v_scale,
@@ -624,12 +625,12 @@ int skv_kv8_read(const uint8_t* codes, int64_t c_stride_b, int64_t c_stride_h, i
  * window > 0 only those with j > p - window or j < sinks:
  *   out[b, t, hq, :] = sum_j exp(scale q[b, hq, t] . k_j) v_j / sum_j exp(scale q[b, hq, t] . k_j)
  * over them, of kv head hq / (q_heads / kv_heads); zeros for a query that sees nothing (p < 0) and for t >= n_b.
- * Keys and values that a query does not see do not reach it, whatever they and their scales hold; a seen block whose
- * scale is NaN or infinite gives NaN. Scores and sums in
- * fp32; with more than 32 rows * q_heads / kv_heads and value scales that are powers of two within 2^12 of one another,
- * probabilities enter their product in f16, else (also beside NaN, or scores past 2^24) with 16 significant bits. out [batch, rows, q_heads, 128] bf16
- * (contiguous, 16-byte aligned). q: rows of 128 bf16 at q + b*q_stride_b + hq*q_stride_h + t*q_stride_t, multiples of
- * 8 elements, 16-byte aligned. c_stride_s at most 2^24. lengths and counts are read when the kernels run. workspace:
+ * Keys and values that a query does not see do not reach it, whatever they and their scales hold, and queries t >= n_b
+ * are not read; a seen block whose scale is NaN or infinite gives NaN. Scores and sums in fp32; with more than 32 rows *
+ * q_heads / kv_heads and value scales that are powers of two within 2^12 of one another, probabilities enter their
+ * product in f16, else (also beside NaN, or scores past 2^24) with 16 significant bits. out [batch, rows, q_heads, 128]
+ * bf16 (contiguous, 16-byte aligned). q: rows of 128 bf16 at q + b*q_stride_b + hq*q_stride_h + t*q_stride_t, multiples
+ * of 8 elements, 16-byte aligned. c_stride_s at most 2^24. lengths and counts are read when the kernels run. workspace:
  * skv_kv8_attn_workspace_bytes bytes (0 for some sizes, and for bad ones), 16-byte aligned, overwritten. */
 int64_t skv_kv8_attn_workspace_bytes(int batch_size, int q_heads, int kv_heads, int rows, int cap, int window,
                                      int sinks);

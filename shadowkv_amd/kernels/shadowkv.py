@@ -1226,10 +1226,46 @@ def _distinct(shape, strides) -> bool:
     return True
 
 
+def _touches(dims, run: int, lo: int, hi: int) -> bool:
+    """Whether bytes [lo, hi) meet one of the runs that begin at the sums of i * stride, i < size, over dims (strides
+    descending, each at least what lies below it takes)."""
+    if not dims:
+        return lo < run and hi > 0
+    (stride, size), rest = dims[0], dims[1:]
+    extent = run + sum([(sz - 1) * st for st, sz in rest])
+    first, last = max(0, (lo - extent) // stride + 1), min(size - 1, (hi - 1) // stride)
+    if last - first > 1:  # (those between lie inside)
+        return True
+    return any([_touches(rest, run, lo - i * stride, hi - i * stride) for i in range(first, last + 1)])
+
+
+def _meets(dims, run: int, d: int) -> bool:
+    """Whether such runs meet the same ones d bytes further."""
+    if not dims:
+        return abs(d) < run
+    (stride, size), rest = dims[0], dims[1:]
+    extent = run + sum([(sz - 1) * st for st, sz in rest])
+    first, last = max(1 - size, (d - extent) // stride + 1), min(size - 1, (d + extent - 1) // stride)
+    return any([_meets(rest, run, d - i * stride) for i in range(first, last + 1)])
+
+
+@functools.lru_cache(maxsize=256)
+def _kv8_overlap(shape, c_strides, s_strides, blocks: int, v8: int, ks: int, vs: int) -> bool:
+    """Whether two caches of one layout, or their scales, share bytes: v8, ks and vs where they begin, in bytes from
+    the keys' codes on."""
+    dims = sorted([(st, sz) for st, sz in zip(c_strides, shape) if sz > 1], reverse=True)
+    s_dims = sorted([(4 * st, sz) for st, sz in zip(s_strides, shape) if sz > 1], reverse=True)
+    if _meets(dims, 128, v8) or _meets(s_dims, 4 * blocks, vs - ks):
+        return True
+    rows = [4 * (b * s_strides[0] + h * s_strides[1]) for b in range(shape[0]) for h in range(shape[1])]
+    return any([_touches(dims, 128, at + row, at + row + 4 * blocks)
+                for at in (ks, vs, ks - v8, vs - v8) for row in rows])
+
+
 @functools.lru_cache(maxsize=256)
 def _kv8_layout(name: str, block: int, shape, strides, dtype, s_shape, s_strides, s_dtype):
-    """Checks the layout of a cache and its scales; returns ((B, H, cap), strides of the codes, of the scales, whether
-    no two elements share memory)."""
+    """Checks the layout of a cache and its scales; returns ((B, H, cap), strides of the codes, of the scales, bytes from
+    the first to the last of each, or None where two elements share memory)."""
     if block not in KV8_BLOCKS:
         raise ValueError(f"block={block} must be one of {KV8_BLOCKS}")
     if dtype != torch.float8_e4m3fn or s_dtype != torch.float32:
@@ -1245,8 +1281,11 @@ def _kv8_layout(name: str, block: int, shape, strides, dtype, s_shape, s_strides
     if len(s_shape) != 3 or s_shape[0] != B or s_shape[1] != H or s_shape[2] < blocks or \
             (s_shape[2] > 1 and s_strides[2] != 1):
         raise ValueError(f"{name} scale {tuple(s_shape)} must be [{B}, {H}, {blocks} or more] with contiguous rows")
-    return ((B, H, cap), c_strides, _strides(s_shape, s_strides, 2),
-            _distinct(shape, strides) and _distinct(s_shape, s_strides))
+    s_strides2 = _strides(s_shape, s_strides, 2)
+    spans = (128 + sum([(n - 1) * st for n, st in zip(shape, c_strides)]),
+             4 * (blocks + sum([(n - 1) * st for n, st in zip(shape, s_strides2)])))
+    return ((B, H, cap), c_strides, s_strides2,
+            spans if _distinct(shape, strides) and _distinct(s_shape, s_strides) else None)
 
 
 def _kv8_cache(codes: torch.Tensor, scale: torch.Tensor, name: str, block: int):
@@ -1286,7 +1325,7 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
     A block's scale is the smallest power of two under which its new rows fit; where it holds older rows (before
     start[b]) it never falls, and they are encoded again where it grows. Infinities become NaN. Nothing else in
     the caches changes."""
-    (B, H, cap), c_strides, s_strides, distinct, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
+    (B, H, cap), c_strides, s_strides, spans, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
     _no_grad("kv8_write", k, v)
     k, k_strides = _rows128(k, "k")
     v, v_strides = _rows128(v, "v")
@@ -1294,12 +1333,17 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
         raise ValueError(f"kv8_write: k {tuple(k.shape)} v {tuple(v.shape)} for caches of [{B}, {H}]")
     if k.get_device() != index or v.get_device() != index:
         raise ValueError("kv8_write: rows and caches must be on one device")
-    if not distinct or k8.data_ptr() == v8.data_ptr() or k_scale.data_ptr() == v_scale.data_ptr():
+    k8p, v8p, ksp, vsp = k8.data_ptr(), v8.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+    n, m = spans or (0, 0)
+    if spans is None or ((-n < v8p - k8p < n or -m < vsp - ksp < m or -m < ksp - k8p < n or -m < vsp - k8p < n or
+                          -m < ksp - v8p < n or -m < vsp - v8p < n) and
+                         _kv8_overlap((B, H, cap), c_strides, s_strides, (cap + block - 1) // block, v8p - k8p,
+                                      ksp - k8p, vsp - k8p)):
         raise ValueError("kv8_write: the caches must not share memory with themselves or each other")
     sp = _kv8_ints(start, "start", B, index)
     cp = None if counts is None else _kv8_ints(counts, "counts", B, index)
-    _call_on(index, "skv_kv8_write", k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, k8.data_ptr(), v8.data_ptr(),
-             *c_strides, k_scale.data_ptr(), v_scale.data_ptr(), *s_strides, sp, cp, B, H, k.shape[2], cap, block)
+    _call_on(index, "skv_kv8_write", k.data_ptr(), *k_strides, v.data_ptr(), *v_strides, k8p, v8p, *c_strides, ksp, vsp,
+             *s_strides, sp, cp, B, H, k.shape[2], cap, block)
 
 
 def _kv8_read(codes, scale, chunk_ids, chunk_size, start, rows, block):

@@ -216,3 +216,37 @@ def test_read_rows_from_the_host(gpu, block):
             want = shadowkv.kv8_read(k8, ks, start, rows, block=block)
             got = shadowkv.kv8_read(c, ks, start, rows, block=block)
             assert torch.equal(got.view(torch.int16), want.view(torch.int16))
+
+
+def test_write_shared_memory(gpu):
+    """Caches that overlap without beginning at the same place are refused; keys, values and scales that lie between
+    one another in a buffer, and share nothing, are written as apart."""
+    _say("kv8_write shared memory")
+    g = torch.Generator().manual_seed(6)
+    B, H, cap, block = 2, 2, 64, 32
+    k, v = _queries(B, H, 40, g, gpu), _queries(B, H, 40, g, gpu)
+    at = _ints([3, 20], gpu)
+    buffer, scales = torch.zeros(B, H, 3 * cap, D, dtype=E4M3, device=gpu), torch.ones(B, H, 8, device=gpu)
+    cut = lambda a: buffer[:, :, a:a + cap]  # noqa: E731
+    for k8, v8, ks, vs in ((cut(0), cut(1), scales[..., :2], scales[..., 2:4]),
+                           (cut(cap), cut(1), scales[..., :2], scales[..., 2:4]),
+                           (cut(0), cut(cap), scales[..., :2], scales[..., 1:3]),
+                           (cut(0), cut(cap), scales[..., 3:5], scales[..., 2:4]),
+                           (buffer[:, :, :2 * cap:2], buffer[:, :, 2:2 * cap + 2:2], scales[..., :2], scales[..., 2:4])):
+        with pytest.raises(ValueError, match="share memory"):
+            shadowkv.kv8_write(k, v, k8, v8, ks, vs, at, block=block)
+    assert buffer.view(torch.uint8).max() == 0 and (scales == 1).all()
+    want = _caches(B, H, cap, block, g, gpu)
+    start = [c.clone() for c in want]
+    shadowkv.kv8_write(k, v, *want, at, block=block)
+    records = torch.zeros(B, H, 2 * cap * D + 32, dtype=torch.uint8, device=gpu)  # a head's codes and scales together
+    per = records.view(E4M3)[..., :2 * cap * D].unflatten(-1, (2, cap, D))
+    tail = records.view(torch.float32)[..., 2 * cap * D // 4:]
+    for k8, v8, ks, vs in ((cut(5), cut(5 + cap), scales[..., 1:3], scales[..., 4:6]),
+                           (buffer[:, :, :2 * cap:2], buffer[:, :, 1:2 * cap + 1:2], scales[..., :2], scales[..., 2:4]),
+                           (per[:, :, 0], per[:, :, 1], tail[..., :2], tail[..., 2:4])):
+        for c, s in zip((k8, v8, ks, vs), start):
+            c.copy_(s) if c.dtype != E4M3 else c.view(torch.uint8).copy_(s.view(torch.uint8))
+        shadowkv.kv8_write(k, v, k8, v8, ks, vs, at, block=block)
+        for c, w in zip((k8, v8, ks, vs), want):
+            assert torch.equal(c.contiguous().view(torch.uint8), w.view(torch.uint8))
