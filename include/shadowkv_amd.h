@@ -602,7 +602,7 @@ int skv_linear_qkv_rope_append(const uint16_t* x, int64_t x_stride, const uint16
  * In each block with a new row, need = the smallest power of two, at least 2^-126, under which the new
  * rows' largest finite magnitude is at most 448; the block's scale becomes need, or, where it holds older rows (of
  * its positions before start[b]), max(scale, need), and those are encoded again where that is larger.
- * Codes are value / scale to nearest even; infinities and NaN become NaN (the format has no infinity).
+ * Codes are value / scale (in fp32) to nearest even; infinities and NaN become NaN (the format has no infinity).
  * Every other code and scale stays as it is. The results do not depend on the order of execution. The two caches'
  * codes and scales share no memory with one another. */
 int skv_kv8_write(const uint16_t* k, int64_t k_stride_b, int64_t k_stride_h, int64_t k_stride_t, const uint16_t* v,

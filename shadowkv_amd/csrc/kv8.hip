@@ -112,6 +112,8 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
   const float was = begun ? *sp : 0.f;
   const float s = fmaxf(was, scale_for(top));
   const float inv = 1.f / s;
+  // (uniform; of a held scale that no write made: the product with the reciprocal would miss ties)
+  const bool divide = (__float_as_uint(s) & 0x7fffffu) != 0;
   const bool again = begun && was < s;
   const float ratio = was * inv;
   uint8_t* dst = a.codes[which] + b * a.c_sb + h * a.c_sh + 8 * c;
@@ -126,6 +128,12 @@ __global__ void __launch_bounds__(kThreads) write_kernel(WriteArgs a) {
         f[2 * e] = skv::bf_lo(v[p][e]) * inv;
         f[2 * e + 1] = skv::bf_hi(v[p][e]) * inv;
       }
+      if (divide)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          f[2 * e] = skv::bf_lo(v[p][e]) / s;
+          f[2 * e + 1] = skv::bf_hi(v[p][e]) / s;
+        }
       *d = encode8(f);
     } else if (again && at < st) {
       const u32x2 old = *d;

@@ -8,7 +8,7 @@ import torch
 from shadowkv_amd import _lib
 from shadowkv_amd.kernels import shadowkv
 
-from .test_gpu_kv8 import BF16, D, E4M3, _caches, _filled, _queries, _say, _see
+from .test_gpu_kv8 import BF16, D, E4M3, _caches, _check_write, _filled, _queries, _say, _see
 
 pytestmark = pytest.mark.gpu
 
@@ -250,3 +250,21 @@ def test_write_shared_memory(gpu):
         shadowkv.kv8_write(k, v, k8, v8, ks, vs, at, block=block)
         for c, w in zip((k8, v8, ks, vs), want):
             assert torch.equal(c.contiguous().view(torch.uint8), w.view(torch.uint8))
+
+
+@pytest.mark.parametrize("block", [16, 64])
+def test_write_beside_any_scale(gpu, block):
+    """New rows in a block whose scale is no power of two (a cache that something else filled) and stays:
+    the nearest code, ties to the even one. Odd scales, whose products with half steps are in bf16."""
+    _say(f"kv8_write beside any scale block={block}")
+    g = torch.Generator().manual_seed(block)
+    H, cap = 120, 64
+    scale = torch.ldexp((2.0 * torch.arange(H) + 3.0).view(1, H, 1), torch.randint(-20, 20, (1, H, 1), generator=g))
+    caches = _caches(1, H, cap, block, g, gpu)
+    for c in caches[2:]:
+        c.copy_(scale.expand(-1, -1, c.shape[2]))
+    ties = torch.arange(17, 32, 2).float() / 16  # half between two codes
+    x = torch.where(torch.rand(1, H, 7, D, generator=g) < 0.7, ties[torch.randint(0, 8, (1, H, 7, D), generator=g)],
+                    torch.randn(1, H, 7, D, generator=g).clamp(-3, 3))
+    x = torch.ldexp(x * scale.unsqueeze(3), torch.randint(-8, 6, x.shape, generator=g)).to(BF16)
+    _check_write(x.to(gpu), -x.to(gpu), caches, [5], None, block)
