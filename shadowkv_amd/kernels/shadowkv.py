@@ -1326,7 +1326,7 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
     start[b]) it never falls, and they are encoded again where it grows. Infinities become NaN. Nothing else in
     the caches changes."""
     (B, H, cap), c_strides, s_strides, spans, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
-    _no_grad("kv8_write", k, v)
+    _no_grad("kv8_write", k, v, k_scale, v_scale)
     k, k_strides = _rows128(k, "k")
     v, v_strides = _rows128(v, "v")
     if k.shape != v.shape or k.shape[0] != B or k.shape[1] != H:
@@ -1348,6 +1348,7 @@ def kv8_write(k, v, k8, v8, k_scale, v_scale, start, counts=None, *, block=64):
 
 def _kv8_read(codes, scale, chunk_ids, chunk_size, start, rows, block):
     (B, H, cap), c_strides, s_strides, _ = _kv8_cache(codes, scale, "codes", block)
+    _no_grad("kv8_read", scale)
     index = scale.get_device()
     if index < 0 or (codes.is_cuda and codes.get_device() != index):
         raise ValueError("the scales must be on a device, and codes that are on one beside them")
@@ -1393,7 +1394,7 @@ def kv8_attn(q, k8, v8, k_scale, v_scale, lengths, counts=None, *, block=64, sca
     read when the kernels run. Queries that see nothing and those past counts[b] give zeros. What a query does
     not see may hold anything, NaN too, in the codes and in their scales. scale: 1 / sqrt(128) by default."""
     (B, H, cap), c_strides, s_strides, _, index = _kv8_pair(k8, v8, k_scale, v_scale, block)
-    _no_grad("kv8_attn", q)
+    _no_grad("kv8_attn", q, k_scale, v_scale)
     q, q_strides = _rows128(q, "q")
     Bq, Hq, T, _ = q.shape
     if Bq != B or Hq % H or q.get_device() != index:

@@ -268,3 +268,24 @@ def test_write_beside_any_scale(gpu, block):
                     torch.randn(1, H, 7, D, generator=g).clamp(-3, 3))
     x = torch.ldexp(x * scale.unsqueeze(3), torch.randint(-8, 6, x.shape, generator=g)).to(BF16)
     _check_write(x.to(gpu), -x.to(gpu), caches, [5], None, block)
+
+
+def test_scales_that_want_a_gradient(gpu):
+    """The operators have no gradient, for scales neither, and say so."""
+    _say("kv8 scales with gradients")
+    g = torch.Generator().manual_seed(1)
+    k8, v8, ks, vs = _caches(1, 2, 64, 32, g, gpu)
+    x, at = _queries(1, 2, 3, g, gpu), _ints([9], gpu)
+    ids = torch.zeros(1, 2, 1, dtype=torch.int64, device=gpu)
+    for s, t in ((ks.clone().requires_grad_(), vs), (ks, vs.clone().requires_grad_())):
+        for call in (lambda: shadowkv.kv8_write(x, x, k8, v8, s, t, at, block=32),
+                     lambda: shadowkv.kv8_attn(x, k8, v8, s, t, at, block=32)):
+            with pytest.raises(ValueError, match="gradient"):
+                call()
+    s = ks.clone().requires_grad_()
+    for call in (lambda: shadowkv.kv8_read(k8, s, 0, 4, block=32),
+                 lambda: shadowkv.kv8_read_chunks(k8, s, ids, 8, block=32)):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    with torch.no_grad():
+        assert shadowkv.kv8_read(k8, s, 0, 4, block=32).shape == (1, 2, 4, D)
