@@ -50,15 +50,16 @@ class KV8Cache(KVCacheBase):
         self.counts = None  # this step's tokens of each sequence, or None: all that were given
         self.incoming = 0
         self.kv_offset = 0  # the host's bound on the longest sequence: padded rows count
+        self.unfinished = 0  # tokens of a step that has not reached the last layer: held, and not in kv_offset yet
 
     def print_stats(self):
         seen = "all" if self.window is None else f"{self.window} + {self.sinks}"
         print(f"KV8 | block {self.block} | seen {seen} | cached {self.kv_offset} of {self.max_length}")
 
     def check_capacity(self, incoming: int = 1):
-        if self.kv_offset + incoming > self.max_length:
-            raise RuntimeError(f"cache capacity exhausted: {self.kv_offset} of {self.max_length} tokens held, "
-                               f"{incoming} new; construct the cache with a larger max_length")
+        if self.kv_offset + self.unfinished + incoming > self.max_length:
+            raise RuntimeError(f"cache capacity exhausted: {self.kv_offset + self.unfinished} of {self.max_length} tokens "
+                               f"held, {incoming} new; construct the cache with a larger max_length")
 
     def advance(self, incoming: int = 1):
         """Host bookkeeping of one step (the device lengths advance inside the step)."""
@@ -79,9 +80,12 @@ class KV8Cache(KVCacheBase):
                            block=self.block)
         if layer_idx == 0:  # (behind the write: one that is refused leaves the lengths)
             self.lengths.add_(incoming if counts is None else counts.clamp(0, incoming))
-            self.counts, self.incoming = counts, incoming
+            if self.unfinished:  # a step that ended before the last layer: its tokens are held
+                self.advance(self.unfinished)
+            self.counts, self.incoming, self.unfinished = counts, incoming, incoming
         if layer_idx == self.num_layers - 1:
-            self.advance(incoming)
+            self.advance(self.unfinished)
+            self.unfinished = 0
 
     def attend(self, query_states: torch.Tensor, layer_idx: int) -> torch.Tensor:
         """Attention of this step's queries [B, Hq, T, 128] over the layer, their own keys in it -> [B, T, Hq, 128];
@@ -107,6 +111,7 @@ class KV8Cache(KVCacheBase):
         self.counts = None
         self.incoming = 0
         self.kv_offset = 0
+        self.unfinished = 0
 
     def get_kv_len(self):
         return self.kv_offset

@@ -1,0 +1,49 @@
+"""The 8-bit cache class's bookkeeping without a GPU: steps that end early, counts, dropped tokens, the capacity."""
+import types
+
+import pytest
+import torch
+
+from shadowkv_amd.kernels import shadowkv
+from shadowkv_amd.models.kvcache import KV8Cache
+
+
+@pytest.fixture
+def cache(monkeypatch):
+    monkeypatch.setattr(shadowkv, "kv8_write", lambda *a, **kw: None)
+    config = types.SimpleNamespace(num_attention_heads=8, num_key_value_heads=2, hidden_size=1024, num_hidden_layers=3)
+    return KV8Cache(config, batch_size=2, max_length=100, device="cpu")
+
+
+def _rows(T):
+    return torch.zeros(2, 2, T, 128, dtype=torch.bfloat16)
+
+
+def _ints(*x):
+    return torch.tensor(x, dtype=torch.int32)
+
+
+def _step(cache, T, counts=None, layers=3):
+    for layer in range(layers):
+        cache.update_kv_cache(_rows(T), _rows(T), layer, counts)
+
+
+def test_steps_that_end_before_the_last_layer_are_counted(cache):
+    _step(cache, 40)
+    assert cache.get_kv_len() == 40
+    _step(cache, 30, layers=2)  # (its tokens are held: the device lengths went on at layer 0)
+    assert cache.lengths.tolist() == [70, 70] and cache.get_kv_len() == 40
+    with pytest.raises(RuntimeError, match="70 of 100 tokens held, 31 new"):
+        cache.check_capacity(31)
+    with pytest.raises(RuntimeError, match="capacity"):
+        cache.update_kv_cache(_rows(31), _rows(31), 0)
+    assert cache.lengths.tolist() == [70, 70]
+    _step(cache, 30)
+    assert cache.lengths.tolist() == [100, 100] and cache.get_kv_len() == 100
+    with pytest.raises(RuntimeError, match="capacity"):
+        cache.check_capacity(1)
+    cache.clear()
+    _step(cache, 60, layers=1)
+    cache.clear()
+    _step(cache, 100)
+    assert cache.get_kv_len() == 100
