@@ -68,13 +68,16 @@ class KV8Cache(KVCacheBase):
     def update_kv_cache(self, new_k_cache: torch.Tensor, new_v_cache: torch.Tensor, layer_idx: int,
                         counts: torch.Tensor | None = None):
         """Append the new tokens [B, H, T, 128] of one layer: the first counts[b] rows of each sequence (device int32
-        [B]; all T without it, and given at layer 0 for the whole step)."""
+        [B]; all T without it). Layer 0's counts are the whole step's: the other layers may be given them too, and
+        theirs are not read."""
         incoming = new_k_cache.shape[-2]
         if layer_idx == 0:
             self.check_capacity(incoming)
             self.start.copy_(self.lengths)
         elif incoming != self.incoming:
             raise ValueError(f"layer {layer_idx} got {incoming} tokens in a step of {self.incoming}")
+        elif counts is not None and self.counts is None:
+            raise ValueError(f"layer {layer_idx} got counts in a step whose layer 0 had none")
         shadowkv.kv8_write(new_k_cache, new_v_cache, self.k8[layer_idx], self.v8[layer_idx], self.k_scale[layer_idx],
                            self.v_scale[layer_idx], self.start, counts if layer_idx == 0 else self.counts,
                            block=self.block)

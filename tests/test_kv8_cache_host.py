@@ -47,3 +47,13 @@ def test_steps_that_end_before_the_last_layer_are_counted(cache):
     cache.clear()
     _step(cache, 100)
     assert cache.get_kv_len() == 100
+
+
+def test_counts_of_later_layers(cache):
+    cache.update_kv_cache(_rows(5), _rows(5), 0)
+    with pytest.raises(ValueError, match="counts"):
+        cache.update_kv_cache(_rows(5), _rows(5), 1, _ints(3, 5))
+    cache.update_kv_cache(_rows(5), _rows(5), 1)
+    cache.clear()
+    _step(cache, 5, _ints(3, 5))
+    assert cache.lengths.tolist() == [3, 5] and cache.get_kv_len() == 5
