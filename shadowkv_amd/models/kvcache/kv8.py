@@ -35,7 +35,7 @@ class KV8Cache(KVCacheBase):
             raise ValueError(f"block={block} must be one of {shadowkv.KV8_BLOCKS}")
         if not 1 <= max_length <= shadowkv.KV8_MAX_TOKENS:
             raise ValueError(f"max_length={max_length} must be 1 to {shadowkv.KV8_MAX_TOKENS}")
-        if (window is not None and window < 1) or sinks < 0 or (sinks and window is None):
+        if (window is not None and not 1 <= window < 2 ** 31) or not 0 <= sinks < 2 ** 31 or (sinks and window is None):
             raise ValueError(f"window={window} sinks={sinks} (a window of at least 1; sinks need one)")
         self.block, self.window, self.sinks = block, window, sinks
 

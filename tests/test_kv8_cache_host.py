@@ -57,3 +57,10 @@ def test_counts_of_later_layers(cache):
     cache.clear()
     _step(cache, 5, _ints(3, 5))
     assert cache.lengths.tolist() == [3, 5] and cache.get_kv_len() == 5
+
+
+def test_windows_that_no_call_takes():
+    config = types.SimpleNamespace(num_attention_heads=8, num_key_value_heads=2, hidden_size=1024, num_hidden_layers=1)
+    for wrong in (dict(window=2 ** 31), dict(window=5, sinks=2 ** 31)):
+        with pytest.raises(ValueError):
+            KV8Cache(config, max_length=64, device="cpu", **wrong)
