@@ -49,7 +49,7 @@ class KV8Cache(KVCacheBase):
         self.start = torch.zeros(batch_size, dtype=torch.int32, device=device)  # where this step's tokens begin
         self.counts = None  # this step's tokens of each sequence, or None: all that were given
         self.incoming = 0
-        self.kv_offset = 0  # the host's bound on the longest sequence: padded rows count
+        self.kv_offset = 0  # the host's bound on the longest sequence: padded rows count (until trim())
         self.unfinished = 0  # tokens of a step that has not reached the last layer: held, and not in kv_offset yet
 
     def print_stats(self):
@@ -89,6 +89,22 @@ class KV8Cache(KVCacheBase):
         if layer_idx == self.num_layers - 1:
             self.advance(self.unfinished)
             self.unfinished = 0
+
+    def trim(self, lengths: torch.Tensor, longest: int):
+        """Between steps: keep the first min(lengths[b], longest) tokens of each sequence (lengths: device int32 [B]; all
+        that it holds if those are fewer) and drop the others: drafted ones that were rejected, or a step that failed on
+        its way. The capacity is counted from `longest` on: cache.lengths with the longest sequence's tokens takes the
+        padding of a ragged batch out of it. A captured trim() takes max_length, and kv_offset is set beside its
+        replays."""
+        if lengths.dtype != torch.int32 or lengths.shape != self.lengths.shape or lengths.device != self.lengths.device:
+            raise ValueError(f"lengths must be {self.batch_size} int32 on {self.lengths.device}, got "
+                             f"{tuple(lengths.shape)} {lengths.dtype} on {lengths.device}")
+        if longest < 0:
+            raise ValueError(f"longest={longest} must not be negative")
+        self.lengths.copy_(torch.minimum(self.lengths, lengths.clamp(0, longest)))
+        self.kv_offset = min(self.kv_offset + self.unfinished, longest)
+        self.unfinished = self.incoming = 0
+        self.counts = None
 
     def attend(self, query_states: torch.Tensor, layer_idx: int) -> torch.Tensor:
         """Attention of this step's queries [B, Hq, T, 128] over the layer, their own keys in it -> [B, T, Hq, 128];

@@ -59,6 +59,32 @@ def test_counts_of_later_layers(cache):
     assert cache.lengths.tolist() == [3, 5] and cache.get_kv_len() == 5
 
 
+def test_trim(cache):
+    _step(cache, 60, _ints(7, 50))
+    cache.trim(cache.lengths, 50)  # (the padding of the prompts)
+    assert cache.lengths.tolist() == [7, 50] and cache.get_kv_len() == 50
+    for _ in range(12):  # five drafted tokens a step, one or two of them kept
+        _step(cache, 5)
+        cache.trim(cache.start + _ints(2, 1), cache.get_kv_len() - 4)
+    assert cache.lengths.tolist() == [31, 62] and cache.get_kv_len() == 62
+    with pytest.raises(ValueError, match="in a step of 0"):
+        cache.update_kv_cache(_rows(5), _rows(5), 1)
+    with pytest.raises(ValueError, match="in a step of 0"):
+        cache.attend(_rows(5), 0)
+    _step(cache, 9, layers=2)
+    cache.trim(cache.start, 62)  # (a step that failed)
+    assert cache.lengths.tolist() == [31, 62] and cache.get_kv_len() == 62
+    cache.trim(_ints(-4, 1000), 100)
+    assert cache.lengths.tolist() == [0, 62] and cache.get_kv_len() == 62
+    cache.trim(cache.lengths, 10)
+    assert cache.lengths.tolist() == [0, 10] and cache.get_kv_len() == 10
+    for wrong in (_ints(1), _ints(1, 2).long(), _ints(1, 2).view(1, 2)):
+        with pytest.raises(ValueError):
+            cache.trim(wrong, 5)
+    with pytest.raises(ValueError):
+        cache.trim(cache.lengths, -1)
+
+
 def test_windows_that_no_call_takes():
     config = types.SimpleNamespace(num_attention_heads=8, num_key_value_heads=2, hidden_size=1024, num_hidden_layers=1)
     for wrong in (dict(window=2 ** 31), dict(window=5, sinks=2 ** 31)):
