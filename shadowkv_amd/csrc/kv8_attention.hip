@@ -8,7 +8,7 @@
 // their way into the matrix cores; a key block's scale multiplies its scores and a value block's scale its
 // probabilities, so no dequantised row is ever formed. Scores, probabilities and sums are fp32. A probability
 // enters the product with the values as two bf16 parts (16 significant bits, an error of 2^-16 where the output's
-// one rounding is 2^-9); with many rows, where the matrix cores are the bound, as one f16 (11 bits, 2^-12, and the
+// one rounding is 2^-8); with many rows, where the matrix cores are the bound, as one f16 (11 bits, 2^-11, and the
 // sum that divides the result takes the same rounded ones), wherever f16 holds the values exactly.
 #include <algorithm>
 #include <cmath>
@@ -144,14 +144,14 @@ __device__ __forceinline__ float sum_of_rows(float x) {
 // ------------------------------------------------------------------------------------------------
 // Few rows: up to 32 of a kv head's query heads and new tokens together (row t * G + g).
 //
-// Bound: HBM, 256 bytes a key. The sequences' keys are cut into chunks of equal length, however different the
-// sequences are (planned on the device from the lengths, so that a captured call follows them), each a workgroup
-// of four waves that take its groups of 32 keys in turn, straight from memory into registers: S^T = K Q^T on
-// v_mfma_f32_16x16x32_bf16 (a row of the queries a column) leaves a lane with 8 keys' scores of one row, which is the
-// second operand of O^T = V^T P^T, whose first is the lane's 8 tokens of one dim: neither probabilities nor
-// values cross lanes. Measured (MI355X, 4 query heads on each of 8 kv heads): 8 sequences of 122880 tokens 306 us, 6.6
-// TB/s; 24 windows of 8192 keys and 64 sinks 74 us, 5.3 TB/s; 5 tokens each of 4 sequences of up to 30011 40 us, 3.9
-// TB/s (two tiles of rows leave two waves a SIMD to hide the loads' latency).
+// Bound: HBM, 256 bytes a key. The sequences' keys are cut into chunks of equal length, however different the sequences
+// are (planned on the device from the lengths, so that a captured call follows them), each a workgroup of four waves
+// that take its groups of 32 keys in turn, straight from memory into registers: S^T = K Q^T on v_mfma_f32_16x16x32_bf16
+// (a row of the queries a column) leaves a lane with 8 keys' scores of one row, which is the second operand of O^T =
+// V^T P^T, whose first is the lane's 8 tokens of one dim: neither probabilities nor values cross lanes. Measured
+// (MI355X, 4 query heads on each of 8 kv heads, both launches): 8 sequences of 122880 tokens 306 us, 6.6 TB/s; 24
+// windows of 8192 keys and 64 sinks 74 us, 5.3 TB/s; 5 tokens each of 4 sequences of up to 30011 41 us, 3.8 TB/s (two
+// tiles of rows leave two waves a SIMD to hide the loads' latency).
 constexpr int kGroup = 32;
 constexpr int kGroupShift = 5;
 constexpr int kMinGroups = 8;   // a chunk's groups of 32 keys, at least
@@ -228,8 +228,8 @@ __global__ void __launch_bounds__(few_threads(kTiles, kWhole), kTiles == 1 ? 4 :
   const int li = lane & 15, grp = lane >> 4;
 
   // Q as the B operand: lane (li, grp) holds row li of a tile, in step s dims 64 (s / 2) + 16 grp + 8 (s % 2) and on.
-  // Rows past the last, and of padding, ride along with the last query (padding's own memory, which may hold anything, is
-  // not read), and give nothing in the end.
+  // Rows past the last, and of padding, ride along with the last query (padding's own memory, which may hold anything,
+  // is not read), and give nothing in the end.
   bf16x8 qf[kTiles][4];
   int p[kTiles];
 #pragma unroll
@@ -541,15 +541,16 @@ __global__ void __launch_bounds__(256) few_join_kernel(Args a) {
 // ------------------------------------------------------------------------------------------------
 // More rows.
 //
-// Bound: the matrix cores (with few rows, HBM). The rows of a kv head are its queries' heads together, row
-// t * G + g, so that a tile of keys serves all of them. A workgroup of four waves (eight) owns 128 (256) rows, 32 a
-// wave, a row a lane, and walks the tiles of 64 keys that any of them sees, or a share of them where there are too few
-// rows to fill the chip. Keys and values are read once a tile, turned into 16 bits (the values transposed) by the
-// threads that read them, and shared through LDS, the next tile on its way meanwhile. Measured (MI355X): 8192 causal
-// tokens of 32 heads over 8, 533 us, 1.03 PFLOP/s where a large bf16 GEMM has 1.22; 2048 tokens behind up to 31285
-// others, 16 heads on each of 2 kv heads, a window of 8192, two sequences, 515 us, 0.94 PFLOP/s. Counters (the prompt):
-// the matrix cores are busy in 46% of the cycles, the vector units in 47%, LDS in 32%, at a clock of 1.9 of 2.4 GHz:
-// the power is the limit, and vector work that hides behind the matrix instructions only in part.
+// Bound: the matrix cores (with few rows, HBM). The rows of a kv head are its queries' heads together, row t * G + g,
+// so that a tile of keys serves all of them. A workgroup of four waves (eight) owns 128 (256) rows, 32 a wave, a row a
+// lane, and walks the tiles of 64 keys that any of them sees, or a share of them where there are too few rows to fill
+// the chip. Keys and values are read once a tile, turned into 16 bits (the values transposed) by the threads that read
+// them, and shared through LDS, the next tile on its way meanwhile. Measured (MI355X): 8192 causal tokens of 32 heads
+// over 8, 547 us, 1.00 PFLOP/s where a large bf16 GEMM has 1.22 (533 to 557 from machine to machine), 1003 us where the
+// values take the form in 16 bits; 2048 tokens behind up to 31285 others, 16 heads on each of 2 kv heads, a window of
+// 8192, two sequences, 532 us, 0.91 PFLOP/s. Counters (the prompt): the matrix cores are busy in 46% of the cycles, the
+// vector units in 47%, LDS in 32%, at a clock of 1.9 of 2.4 GHz: the power is the limit, and vector work that hides
+// behind the matrix instructions only in part.
 constexpr int kTile = 64;
 constexpr int kTileShift = 6;
 constexpr int kRowsWave = 32;
@@ -603,7 +604,8 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
   i /= BH;
   // Consecutive workgroups go to the XCDs in turn: one (sequence, kv head) stays with its XCDs, whose L2 holds its
   // keys, while the chip takes on one set of workgroups; for the next set the sequences, whose work differs, change
-  // places (four of 2000 to 8000 tokens: 458 -> 408 us; at every tile 387, but two windowed pieces 512 -> 531).
+  // places (1024 tokens of each of four sequences of 2000 to 8000: 412 us without, 388 so, 398 at every tile; two
+  // pieces of 2048 under a window: 476, 481, 510; sequences of one length lose 1%).
   bh = (bh / a.H + static_cast<int>(static_cast<int64_t>(i) * BH / (2048 / kWaves))) % a.B * a.H + bh % a.H;
   const int split = i % a.splits;
   const int rt = a.rtiles - 1 - i / a.splits;  // the longest first
@@ -1172,16 +1174,21 @@ struct Plan {
 
 // Tiles of 64 keys from which workgroups of 8 waves take the rows, if more than 128 and enough for every CU: a thread
 // then turns half as many codes into 16 bits, but a tile's barrier holds a whole CU, and a CU without a second
-// workgroup waits for the longest (MI355X, us, 4 waves / 8: 4 query heads on each of 8 kv heads, 2000 tokens of a
-// prompt 38 / 45, 4096 110 / 105, 16384 1389 / 1365, 4 sequences' 100 tokens on 30000 keys 171 / 160; three ragged
-// prompts of 4000 on 4 heads, 192 workgroups of 8, 90 / 110; with up to 128 rows the added waves have none: 9 tokens
-// 50 / 56).
+// workgroup waits for the longest (MI355X, us on the device, 4 waves / 8; 4 query heads on each of 8 kv heads: 2000
+// tokens of a prompt 57 / 65, 4096 164 / 154, 16384 2116 / 2064, 4 sequences' 100 tokens on 30000 keys 250 / 235; three
+// ragged prompts of 4000 on 4 heads, 192 workgroups of 8, 90 / 111; with up to 128 rows the added waves have none: 9
+// tokens of 4 sequences on 30000 67 / 84. It loses where 192 workgroups have the same work each: 24 sequences' 64
+// tokens on 16000 keys 518 / 477, but on 667 to 16000 352 / 422).
 constexpr int kLongTiles = 40;
 
 // Shares of a row tile's keys, of at least 4 tiles, where the workgroups alone would leave part of the chip idle: as
-// many as make the walk and the join together shortest. A workgroup walks a tile in about 1.1 us; a share's partial
-// rows, written and read, cost 1 KB each, and the join 5 us (MI355X, us, one share / as many as fit: 64 tokens on 8000
-// keys 140 / 24, on 2000 33 / 16; 1000 tokens of a prompt 21 / 39, 500 14 / 27).
+// many as make the walk and the join together shortest. A share's partial rows, written and read, cost 1 KB each, and
+// the join 5 us. A workgroup walks a tile in 1.2 us alone on its CU and in 2.0 beside another: taken as 1.1, which
+// leaves one share where two would only put workgroups beside one another (1000 tokens on 2000 keys 51 us, with 1.2 in
+// two shares 74). Measured (MI355X, us on the device, one share / as many as fit / these; 4 query heads on each of 8 kv
+// heads): 64 tokens on 8000 keys 156 / 34 / 36, on 2000 50 / 24 / 24; a prompt of 1000 tokens 32 / 57 / 32, of 500 21 /
+// 39 / 21; 471 on 100315 1915 / 809 / 832. It errs where two shares just fill the chip: seven sequences' 520 tokens on
+// 3064 keys, 7 heads on one, 71 / 81 / 81.
 int shares(int64_t tiles, int64_t wgs, int64_t resident, double rows) {
   const double walk = 1.1 * static_cast<double>(tiles), each = 2e-4 * rows;
   const int64_t most = std::min<int64_t>(resident / wgs, tiles / 4);
