@@ -62,8 +62,11 @@ class KV8Cache(KVCacheBase):
                                f"held, {incoming} new; construct the cache with a larger max_length")
 
     def advance(self, incoming: int = 1):
-        """Host bookkeeping of one step (the device lengths advance inside the step)."""
+        """Host bookkeeping of one step (the device lengths advance inside the step): a replayed one, or one that is
+        complete without this cache's last layer."""
         self.kv_offset += incoming
+        if incoming == self.unfinished:
+            self.unfinished = 0
 
     def update_kv_cache(self, new_k_cache: torch.Tensor, new_v_cache: torch.Tensor, layer_idx: int,
                         counts: torch.Tensor | None = None):
@@ -88,7 +91,6 @@ class KV8Cache(KVCacheBase):
             self.counts, self.incoming, self.unfinished = counts, incoming, incoming
         if layer_idx == self.num_layers - 1:
             self.advance(self.unfinished)
-            self.unfinished = 0
 
     def trim(self, lengths: torch.Tensor, longest: int):
         """Between steps: keep the first min(lengths[b], longest) tokens of each sequence (lengths: device int32 [B]; all

@@ -49,6 +49,15 @@ def test_steps_that_end_before_the_last_layer_are_counted(cache):
     assert cache.get_kv_len() == 100
 
 
+def test_steps_that_are_advanced_by_hand(cache):
+    for n in range(5):  # (the last layer is another cache's)
+        _step(cache, 20, layers=2)
+        cache.advance(20)
+        assert cache.get_kv_len() == 20 * (n + 1) and cache.unfinished == 0
+    with pytest.raises(RuntimeError, match="capacity"):
+        cache.check_capacity(1)
+
+
 def test_counts_of_later_layers(cache):
     cache.update_kv_cache(_rows(5), _rows(5), 0)
     with pytest.raises(ValueError, match="counts"):
