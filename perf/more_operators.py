@@ -176,8 +176,8 @@ def _table(case, totals, gen, width):
 
 def prepare(case, seed):
     gen = torch.Generator(device=DEV).manual_seed(seed)
+    st = dict(case=case, cu=_ints(_begins(case)))
     n, totals, counts = _rows(case), _totals(case), _counts(case)
-    st = dict(case=case, rows=n, cu=_ints(_begins(case)))
     if case["kind"] == "prompt":
         H, G = case["heads"], case["group"]
         st["q"], st["k"], st["v"] = _qkv(n, (H * G, H, H), gen, (1.2, 1.0, 0.6), (0, 0.5, 0))
@@ -305,7 +305,7 @@ def _own(st):
     case = st["case"]
     if case["kind"] == "tables":
         step = shadowkv.paged_reserve(st["lengths"], st["counts"], st["table"], st["held"], st["free_pages"],
-                                      st["free_count"], rows=st["rows"], page=case["page"])
+                                      st["free_count"], rows=_rows(case), page=case["page"])
         shadowkv.paged_release(st["lengths"], st["lengths"], st["table"], st["held"], st["free_pages"],
                                st["free_count"], page=case["page"])
         return list(step)
