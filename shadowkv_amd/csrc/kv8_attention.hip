@@ -180,9 +180,10 @@ __device__ __forceinline__ int chunk_groups(const Args& a, int lane) {
   int64_t total = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int t = b0 + lane < a.B ? few_groups(a, b0 + lane).total : 0;
-    total += __builtin_amdgcn_readlane(skv::wave_inclusive_scan(t), 63);
+    total += skv::wave_total(t);  // (64 sequences of 2^30 tokens have 2^31 groups)
   }
-  return static_cast<int>(max(static_cast<int64_t>(kMinGroups), (total * a.H + a.target - 1) / a.target));
+  return static_cast<int>(min(max(static_cast<int64_t>(kMinGroups), (total * a.H + a.target - 1) / a.target),
+                              static_cast<int64_t>(1 << 30)));
 }
 
 // Chunk i of all sequences' (false past the last).

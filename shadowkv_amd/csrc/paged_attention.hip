@@ -197,10 +197,11 @@ __device__ __forceinline__ Seq seq_or_none(const Args& a, int b) { return b < a.
 // The chunk length, wave-uniform: the sequences' groups dealt over the workgroups to aim for. total0: the lane's
 // sequence's, of the first 64.
 __device__ __forceinline__ int chunk_groups(const Args& a, int lane, int total0) {
-  int64_t total = __builtin_amdgcn_readlane(skv::wave_inclusive_scan(total0), 63);
-  for (int b0 = 64; b0 < a.B; b0 += 64)
-    total += __builtin_amdgcn_readlane(skv::wave_inclusive_scan(few_groups(a, seq_or_none(a, b0 + lane)).total), 63);
-  return static_cast<int>(max(static_cast<int64_t>(kMinGroups), (total * a.H + a.target - 1) / a.target));
+  int64_t total = skv::wave_total(total0);  // (64 sequences of 2^30 tokens have 2^31 groups)
+  for (int b0 = 64; b0 < a.B; b0 += 64) total += skv::wave_total(few_groups(a, seq_or_none(a, b0 + lane)).total);
+  // (at most what no sequence has)
+  return static_cast<int>(min(max(static_cast<int64_t>(kMinGroups), (total * a.H + a.target - 1) / a.target),
+                              static_cast<int64_t>(1 << 30)));
 }
 
 __device__ __forceinline__ Seq lane_seq(const Seq& s, int l) {

@@ -182,6 +182,12 @@ __device__ __forceinline__ int wave_inclusive_scan(int v) {
   return v;
 }
 
+// Sum over the wave of counts below 2^31, which together may pass it.
+__device__ __forceinline__ int64_t wave_total(int v) {
+  const int high = __builtin_amdgcn_readlane(wave_inclusive_scan(v >> 16), 63);
+  return (static_cast<int64_t>(high) << 16) + __builtin_amdgcn_readlane(wave_inclusive_scan(v & 0xffff), 63);
+}
+
 // Exclusive prefix sum over the whole workgroup. `scratch` needs blockDim.x/64 + 1 ints of LDS.
 // Returns the exclusive prefix for this thread; *total receives the workgroup sum.
 __device__ __forceinline__ int block_exclusive_scan(int v, int* scratch, int* total) {

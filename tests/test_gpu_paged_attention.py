@@ -321,6 +321,18 @@ def test_pool_of_more_than_2_to_the_31_elements(gpu):
     assert torch.equal(_run_paged(far, gpu), _run_paged(c, gpu))
 
 
+def test_sequences_of_2_to_the_31_groups_together(gpu):
+    """64 sequences of as many tokens as a table can hold, all of them one page, over and over: the mean of equal values.
+    (Sums of ones, below 2^24 in a wave: exact.)"""
+    page, width = 256, shadowkv.PAGED_MAX_TOKENS // 256
+    table = torch.zeros(1, width, dtype=torch.int32, device=gpu).expand(64, width)
+    kp = torch.randn(1, 1, page, 128, generator=torch.Generator().manual_seed(0)).to(BF16).to(gpu)
+    vp = torch.ones_like(kp)
+    q = torch.zeros(64, 1, 128, dtype=BF16, device=gpu)
+    out = shadowkv.paged_attn(q, kp, vp, table, _ints([shadowkv.PAGED_MAX_TOKENS] * 64, gpu))
+    assert bool((out == 1).all())
+
+
 def test_the_same_bits_each_time_and_on_another_stream(gpu):
     for counts, max_new in (([1, 1, 3], 3), ([90, 1, 200], None)):
         c = _paged_case(gpu, [2000, 5000, 900], counts, 2, 4, 64, seed=3)
