@@ -86,9 +86,9 @@ class PagedKVCache(KVCacheBase):
                         counts: torch.Tensor | None = None, max_new: int | None = None):
         """Append the new tokens of one layer: T of each sequence, [batch_size, H, T, 128], or with counts (device int32
         [batch_size]) packed rows [1, H, N, 128], counts[b] of sequence b behind those of the sequences before it; rows
-        behind the last are padding. A sequence that lacks pages is left as it is (refused()). max_new: the host's bound on
-        counts (default: N), by which the capacity is counted; a sequence with more gets zeros from the attention. Layer
-        0's counts are the whole step's: the other layers may be given them too, and theirs are not read."""
+        behind the last are padding. max_new: the host's bound on counts (default: N), by which the capacity is counted. A
+        sequence that lacks pages, or has more new tokens than max_new, is left as it is (refused()). Layer 0's counts are
+        the whole step's: the other layers may be given them too, and theirs are not read."""
         k, v = self._packed(new_k_cache), self._packed(new_v_cache)
         rows = k.shape[0]
         if layer_idx == 0:
@@ -106,9 +106,13 @@ class PagedKVCache(KVCacheBase):
                     raise ValueError(f"counts must be {self.batch_size} int32, got {tuple(counts.shape)} {counts.dtype}")
                 self.asked.copy_(counts)
             self.start.copy_(self.lengths)
+            # (one with more new tokens than the bound is left as it is: no length is the reserve's sign for that; one
+            # with more than there are rows is by itself)
+            lengths = self.lengths
+            if counts is not None and new < rows:
+                lengths = lengths.masked_fill(self.asked > new, -1)
             self.cu, self.totals, self.slots = shadowkv.paged_reserve(
-                self.lengths, self.asked, self.table, self.held, self.free_pages, self.free_count, rows=rows,
-                page=self.page)
+                lengths, self.asked, self.table, self.held, self.free_pages, self.free_count, rows=rows, page=self.page)
             # (here, where a replay's go too: a captured step's totals are its graph's own)
             torch.eq(self.totals, 0, out=self.unserved)
         elif rows != self.incoming:
@@ -123,8 +127,9 @@ class PagedKVCache(KVCacheBase):
             self.advance(self.unfinished)
 
     def refused(self) -> torch.Tensor:
-        """Which sequences' tokens the last step (an eager or a replayed one) did not take, for lack of pages (device bool
-        [batch_size]): their outputs are zeros. They can be given again when others have ended."""
+        """Which sequences' tokens the last step (an eager or a replayed one) did not take (device bool [batch_size]), for
+        lack of pages or as more than its max_new: their outputs are zeros. They can be given again, when others have ended
+        or in pieces."""
         return self.unserved & (self.asked > 0)
 
     def trim(self, lengths: torch.Tensor, longest: int):

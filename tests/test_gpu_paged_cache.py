@@ -200,3 +200,53 @@ def test_refused_follows_replays(gpu):
         lengths = [n + (0 if refused else T) for n in lengths]
         assert cache.refused().tolist() == [bool(refused)] * B and cache.lengths.tolist() == lengths, (T, how)
         cache.kv_offset, cache.unfinished = max(lengths), 0
+
+
+def test_captured_packed_steps_follow_the_counts(gpu):
+    """A captured step of packed rows, replayed while its counts change, stores and answers what an eager one does; a
+    sequence with more new tokens than the host's bound is left as it is, answered with zeros and refused()."""
+    g = torch.Generator().manual_seed(2)
+    B, N, most = 3, 12, 5
+    made = [_made(gpu, B, 256, page=16, pages=40) for _ in range(2)]
+    x = [_inputs(1, N, g, gpu) for _ in range(L)]
+    counts = torch.zeros(B, dtype=torch.int32, device=gpu)
+    rows = torch.arange(N, device=gpu)
+
+    def step(cache, attn):
+        ends = counts.cumsum(0)
+        b = torch.searchsorted(ends, rows, right=True).clamp(max=B - 1)
+        pos = (cache.lengths[b] + rows - (ends - counts)[b]).clamp(0, 255).view(1, N)
+        return [attn.prefill(*x[layer], pos, layer, counts=counts, max_new=most) for layer in range(L)]
+
+    for cache, attn, _ in made:
+        step(cache, attn)
+        cache.clear()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with capture_graph(graph, gpu):
+        outs = step(*made[0][:2])
+    made[0][0].clear()
+    lengths = [0] * B
+    for now in ([5, 2, 3], [1, 1, 1], [0, 5, 5], [6, 2, 4], [1, 7, 4], [4, 4, 4], [0, 0, 12], [2, 1, 0]):
+        counts.copy_(torch.tensor(now, dtype=torch.int32))
+        for t in (t for layer in x for t in layer):
+            t.normal_()
+        graph.replay()
+        want = step(*made[1][:2])
+        torch.cuda.synchronize()
+        over = [n > most for n in now]
+        lengths = [n + (0 if o else c) for n, c, o in zip(lengths, now, over)]
+        for a, b in zip(outs, want):
+            assert torch.equal(a, b)
+            for i, o in enumerate(over):
+                mine = a[0, sum(now[:i]):sum(now[:i + 1])]
+                assert not mine.any() if o else not len(mine) or mine.any()
+        for cache, _, _ in made:
+            assert cache.lengths.tolist() == lengths and cache.refused().tolist() == over, now
+        for name in ("table", "held", "free_count", "start"):
+            assert torch.equal(getattr(made[0][0], name), getattr(made[1][0], name)), name
+        for b in range(B):
+            for layer in range(L):
+                for p, r in zip(made[0][0].get_kv(layer, b, lengths[b]), made[1][0].get_kv(layer, b, lengths[b])):
+                    assert torch.equal(p, r)
+        assert max(lengths) <= made[1][0].get_kv_len()

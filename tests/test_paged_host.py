@@ -248,3 +248,22 @@ def test_bookkeeping(cache):
     assert cache.refused().tolist() == [True, False] and cache.lengths.tolist() == [30, 68]
     cache.clear()
     assert cache.free_count.item() == 8 and cache.table.eq(-1).all() and cache.get_kv_len() == 0
+
+
+def test_more_new_tokens_than_the_host_said(cache):
+    """Such a sequence is left as it is and known to refused(); the others' rows keep their places, and no length passes
+    the host's bound."""
+    _step(cache, 9, [4, 5], max_new=5)
+    _step(cache, 12, [7, 5], max_new=5)
+    assert cache.refused().tolist() == [True, False] and cache.totals.tolist() == [0, 10]
+    assert cache.lengths.tolist() == [4, 10] and cache.held.tolist() == [1, 1] and cache.get_kv_len() == 10
+    assert cache.cu.tolist() == [0, 7, 12] and cache.slots[:7].eq(-1).all() and cache.slots[7:].ge(0).all()
+    assert cache.start.tolist() == [4, 5]
+    cache.trim(cache.start, 5)
+    assert cache.lengths.tolist() == [4, 5]
+    _step(cache, 12, [7, 5], max_new=7)
+    assert not cache.refused().any() and cache.lengths.tolist() == [11, 10] and cache.get_kv_len() == 12
+    for _ in range(40):
+        _step(cache, 2, [1, 1], max_new=1)
+    _step(cache, 40, [1, 39], max_new=1)
+    assert cache.lengths.tolist() == [52, 50] and int(cache.lengths.max()) <= cache.get_kv_len()
