@@ -665,7 +665,9 @@ int skv_paged_reserve(const int32_t* lengths, const int32_t* counts, int32_t* ta
 /* Sequence b keeps its first min(lengths[b], keep[b]) tokens, its new length; the pages behind those (all that it holds
  * behind, also ones that skv_paged_reserve took for tokens that never came) go back to the free ones, in the order
  * that undoes a skv_paged_reserve of the same sequences, and their table entries become -1. keep[b] < 0: the sequence is
- * left as it is. keep may be lengths. Pages that free_cap has no room for are dropped. */
+ * left as it is. keep may be lengths. Entries below 0 are no pages: they are cleared and not given back. A page that more
+ * than one sequence names is given back with each, and would be free twice: its entries are set to -1 before, in all
+ * but the last of them. Pages that free_cap has no room for are dropped. */
 int skv_paged_release(int32_t* lengths, const int32_t* keep, int32_t* table, int64_t table_stride, int width,
                       int32_t* held, int32_t* free_pages, int free_cap, int32_t* free_count, int batch_size, int page,
                       void* stream);

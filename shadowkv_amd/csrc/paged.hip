@@ -167,6 +167,8 @@ __global__ void __launch_bounds__(256) slots_kernel(Pages g, const int32_t* cu, 
   slots[r] = total > 0 ? slot_of(g.table[lo * g.stride + (at >> g.shift)], at, g.shift) : -1;
 }
 
+// From the last sequence's last page to the first one's first, which comes to lie on top. Entries below zero are no pages:
+// they are cleared and not given back.
 __global__ void __launch_bounds__(kSeqs) release_kernel(Pages g, int32_t* lengths, const int32_t* keep) {
   __shared__ uint32_t part[kSeqs / 64];
   __shared__ uint32_t page_end[kSeqs];
@@ -174,42 +176,37 @@ __global__ void __launch_bounds__(kSeqs) release_kernel(Pages g, int32_t* length
   constexpr uint32_t kBound = 0x7fffffffu;
   const int tid = threadIdx.x;
   const int count = min(max(g.free_count[0], 0), g.cap);
-  uint32_t all = 0;
-  // The first walk counts, the second gives back: the lowest sequence's first page comes to lie on top.
-  for (int pass = 0; pass < 2; ++pass) {
-    uint32_t before = 0;
-    for (int b0 = 0; b0 < g.B; b0 += kSeqs) {
-      const int b = b0 + tid, n = min(g.B - b0, kSeqs);
-      const bool is = b < g.B;
-      const int k = is ? keep[b] : -1, left = is ? min(max(lengths[b], 0), k) : 0;
-      const int have = is ? min(max(g.held[b], 0), g.width) : 0;
-      const int stay = k < 0 ? have : min(have, pages_of(left, g.shift));
-      uint32_t total;
-      const uint32_t upto = min(before + scan_to(static_cast<uint32_t>(have - stay), kBound, part, &total), kBound);
-      const uint32_t end = min(before + total, kBound);
-      if (pass == 1) {
-        page_end[tid] = upto;
-        first[tid] = stay;
-        if (k >= 0) {
-          lengths[b] = left;
-          if (stay < have) g.held[b] = stay;
-        }
-        __syncthreads();
-        for (uint32_t i = before + tid; i < end; i += kSeqs) {
-          const int s = find(page_end, n, i);
-          int32_t* entry = g.table + (b0 + s) * g.stride + first[s] + (i - (s ? page_end[s - 1] : before));
-          const int64_t to = static_cast<int64_t>(count) + all - 1 - i;
-          if (to < g.cap) g.free_pages[to] = *entry;
-          *entry = -1;
-        }
-        __syncthreads();
-      }
-      before = end;
+  int64_t top = count;
+  for (int b0 = (g.B - 1) / kSeqs * kSeqs; b0 >= 0; b0 -= kSeqs) {
+    const int b = b0 + tid, n = min(g.B - b0, kSeqs);
+    const bool is = b < g.B;
+    const int k = is ? keep[b] : -1, left = is ? min(max(lengths[b], 0), k) : 0;
+    const int have = is ? min(max(g.held[b], 0), g.width) : 0;
+    const int stay = k < 0 ? have : min(have, pages_of(left, g.shift));
+    uint32_t total;
+    page_end[tid] = scan_to(static_cast<uint32_t>(have - stay), kBound, part, &total);
+    first[tid] = stay;
+    if (k >= 0) {
+      lengths[b] = left;
+      if (stay < have) g.held[b] = stay;
     }
-    all = before;
+    __syncthreads();
+    for (int64_t end = total; end > 0; end -= kSeqs) {
+      const int64_t i = end - 1 - tid;
+      int32_t id = -1;
+      if (i >= 0) {
+        const int s = find(page_end, n, static_cast<uint32_t>(i));
+        int32_t* entry = g.table + (b0 + s) * g.stride + first[s] + (i - (s ? page_end[s - 1] : 0));
+        id = *entry;
+        *entry = -1;
+      }
+      uint32_t pages;
+      const int64_t to = top + scan_to(id >= 0 ? 1u : 0u, kBound, part, &pages) - 1;
+      if (id >= 0 && to < g.cap) g.free_pages[to] = id;
+      top += pages;
+    }
   }
-  if (tid == 0 && all)
-    g.free_count[0] = static_cast<int>(min(static_cast<int64_t>(count) + all, static_cast<int64_t>(g.cap)));
+  if (tid == 0 && top > count) g.free_count[0] = static_cast<int>(min(top, static_cast<int64_t>(g.cap)));
 }
 
 struct WriteArgs {

@@ -1482,8 +1482,10 @@ def paged_reserve(lengths, counts, table, held, free_pages, free_count, *, rows,
 def paged_release(lengths, keep, table, held, free_pages, free_count, *, page=64):
     """Each sequence keeps its first min(lengths[b], keep[b]) tokens (its new length) and gives back the pages behind
     them: rejected drafts, a step that failed, a sequence that ended (keep 0). keep[b] < 0: it is left as it is. Their
-    table entries become -1, and they lie among the free ones as before the paged_reserve that took them. All int32 on
-    the device and updated in place but keep, which may be lengths itself. free_pages needs room for every page."""
+    table entries become -1, and they lie among the free ones as before the paged_reserve that took them. Entries below 0
+    are not given back; a page that more than one sequence names would be with each: set its entries to -1 before, in all
+    but the last of them. All int32 on the device and updated in place but keep, which may be lengths itself. free_pages
+    needs room for every page."""
     index, B, state = _page_state(table, held, free_pages, free_count, page)
     _call_on(index, "skv_paged_release", _ints(lengths, "lengths", (B,), index), _ints(keep, "keep", (B,), index),
              *state, page)

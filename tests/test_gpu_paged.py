@@ -130,6 +130,29 @@ def test_counts_out_of_range_stay_in_bounds(gpu):
     assert guard.tolist() == [11] * 16 + free.tolist() + [11] * 11 + [-1] * 8 + [11] * 24
 
 
+@pytest.mark.parametrize("B,most,page", [(1, 90, 16), (7, 400, 16), (30, 3000, 16), (1500, 60, 16), (64, 900, 256)])
+def test_pages_that_do_not_exist_are_not_given_back(gpu, B, most, page):
+    """Entries below zero among a sequence's pages (keys that no query sees) are no pages: those around them come back in
+    their order, and what is reserved then has a place for every token."""
+    rng = random.Random(B)
+    lengths = [rng.randrange(1, most) for _ in range(B)]
+    st = State(lengths, -(-most // page) + 2, page, 9, rng, gpu)
+    for b in range(B):
+        for i in range(st.held[b]):
+            if rng.random() < (0.3 if b % 2 else 0.02) or b == i == 0:
+                st.table[b][i] = rng.choice([-1, -2 ** 31])
+    st.t_table.copy_(_ints(st.table, gpu))
+    st.total -= sum(x < 0 for b in range(B) for x in st.table[b][:st.held[b]])
+    for keep in ([rng.choice([-1, 0, n // 2, n]) for n in lengths], [0] * B):
+        shadowkv.paged_release(st.t_lengths, _ints(keep, gpu), *st.args(), page=page)
+        ref.release(st.lengths, keep, st.table, st.held, st.free, page)
+        st.free = [p for p in st.free if p >= 0]
+        st.check()
+    assert len(st.free) == st.total
+    totals = _step(st, [2] * B, 2 * B, gpu)
+    assert sum(n == 2 for n in totals) == min(B, st.total)
+
+
 def test_captured_step_follows_the_lengths(gpu):
     """A captured reserve with its advance, replayed beside eager work, gives what the lists give."""
     rng = random.Random(3)
