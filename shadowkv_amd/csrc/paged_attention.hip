@@ -717,8 +717,11 @@ struct Cut {
 // The shares, wave-uniform: all row tiles' tiles dealt over the workgroups that the chip holds at once; a little longer
 // where there are few row tiles and their shares would need a second round of workgroups (19 row tiles of 1917 tiles in 14
 // shares, 266 for 256 workgroups). s, w: the lane's sequence's, of the first 64.
+// The join makes the same plan again: every step of it is rounded by itself, so that no compiler's choice of fused ones in
+// either kernel tells them apart.
 template <bool kPaged, int kRowsTile>
 __device__ __forceinline__ Share share_tiles(const Args& a, int lane, const Seq& s, const Work& w) {
+#pragma clang fp contract(off)
   // (few tiles: the way past the rest, which costs the smallest calls 3 us)
   if (!a.splits || (a.B <= 64 && !__any(w.tiles >= kMinTiles + kShareGain))) return {1, 1 << 30};
   constexpr float kAtOnce = resident(kRowsTile);
@@ -733,7 +736,8 @@ __device__ __forceinline__ Share share_tiles(const Args& a, int lane, const Seq&
   // Shares of n tiles for one walk of t: worth it where t - n is above kShareGain + r t / n.
   const float r = rts * kRowsTile / kGainRows;
   const auto shares = [&](float n) __attribute__((always_inline)) {
-    n = ceilf(fmaxf(fmaxf(n, kMinTiles), 2.f * r));
+#pragma clang fp contract(off)
+    n = fminf(ceilf(fmaxf(fmaxf(n, kMinTiles), 2.f * r)), 1e9f);
     return Share{static_cast<int>(n), static_cast<int>(fminf(ceilf((n + kShareGain) / (1.f - r / n)), 1e9f))};
   };
   Share share = shares(total * static_cast<float>(a.H) / kAtOnce);

@@ -321,6 +321,21 @@ def test_pool_of_more_than_2_to_the_31_elements(gpu):
     assert torch.equal(_run_paged(far, gpu), _run_paged(c, gpu))
 
 
+@pytest.mark.parametrize("n", [37, 130])
+def test_shares_of_plans_past_2_to_the_24_tiles(gpu, n):
+    """Row tiles of sequences of some 2^24 tokens, each a page of its own over and over: the plan's sums are rounded, and the
+    join finds the shares that the kernel made. (Equal values: sums of multiples of two below 2^24, exact.)"""
+    page, width, B = 256, 2 ** 16, 7
+    table = torch.arange(B, dtype=torch.int32, device=gpu).unsqueeze(1).expand(B, width).contiguous()
+    value = 1 + torch.arange(B, device=gpu) / 8
+    kp = torch.randn(B, 1, page, 128, generator=torch.Generator().manual_seed(0)).to(BF16).to(gpu)
+    vp = value.to(BF16).view(B, 1, 1, 1).expand(B, 1, page, 128).contiguous()
+    q = torch.zeros(B * n, 32, 128, dtype=BF16, device=gpu)
+    lengths = [2 ** 24 - 12345 * b * b for b in range(B)]
+    out = shadowkv.paged_attn(q, kp, vp, table, _ints(lengths, gpu), _ints(_cu([n] * B), gpu), max_new=n)
+    assert torch.equal(out.float(), value.repeat_interleave(n).view(-1, 1, 1).expand(-1, 32, 128))
+
+
 def test_sequences_of_2_to_the_31_groups_together(gpu):
     """64 sequences of as many tokens as a table can hold, all of them one page, over and over: the mean of equal values.
     (Sums of ones, below 2^24 in a wave: exact.)"""
