@@ -104,8 +104,12 @@ __device__ __forceinline__ float add_pair(uint32_t pair, float x) {
                                          false);
 }
 
-// 2^x, x <= 0, and never zero: an infinity stays one.
-__device__ __forceinline__ float factor(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 1.17549435e-38f); }
+// x * f, f at most 1: an infinity stays one, also where f has become zero.
+__device__ __forceinline__ f32x4 lowered(f32x4 x, float f) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) x[r] = __builtin_fabsf(x[r]) == INFINITY ? x[r] : x[r] * f;
+  return x;
+}
 
 // x * scale - ref, the product rounded as the reference's was.
 __device__ __forceinline__ float behind(float x, float scale, float ref) {
@@ -385,11 +389,11 @@ __global__ void __launch_bounds__(few_threads(kWhole), !kWhole && kTiles == 1 ? 
         mx = max_of_rows(mx);
         if (__any(mx > m[y])) {  // wave-uniform
           const float mn = fmaxf(m[y], mx);
-          const float f = mn == -INFINITY ? 1.f : factor(m[y] - mn);
+          const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[y] - mn);
           m[y] = mn;
           l[y] *= f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[y][e] *= f;
+          for (int e = 0; e < 8; ++e) o[y][e] = lowered(o[y][e], f);
         }
         const float ref = m[y] == -INFINITY ? 0.f : m[y];
 #pragma unroll
@@ -503,10 +507,10 @@ __global__ void __launch_bounds__(few_threads(kWhole), !kWhole && kTiles == 1 ? 
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) {
         // (a wave that saw only -inf, beside one that saw more, adds nothing)
-        const float f = factor(m_lds[w][g] - ref);
+        const float f = __builtin_amdgcn_exp2f(m_lds[w][g] - ref);
         const float lw = top > -INFINITY && m_lds[w][g] == -INFINITY ? 0.f : l_lds[w][g];
         lsum += f * lw;
-        sum += f * *reinterpret_cast<const f32x4*>(&o_lds[w][g][d]);
+        sum += lowered(*reinterpret_cast<const f32x4*>(&o_lds[w][g][d]), f);
       }
       if (final_) {
         // (a sum of zero: it sees nothing)
@@ -546,7 +550,7 @@ __device__ __forceinline__ void join_parts(const float* ws_o, const float* ws_ml
 #pragma unroll 4
   for (int i = s; i < n; i += 8) {
     const int64_t at = first + i * stride;
-    acc += factor(ws_ml[2 * at] - ref) * *reinterpret_cast<const f32x4*>(ws_o + at * kD + 4 * d);
+    acc += lowered(*reinterpret_cast<const f32x4*>(ws_o + at * kD + 4 * d), __builtin_amdgcn_exp2f(ws_ml[2 * at] - ref));
   }
   acc_lds[s][d] = acc;
   __syncthreads();
@@ -1461,7 +1465,7 @@ __global__ void __launch_bounds__(256) rows_join_kernel(Args a, int few_wgs) {
           const int64_t p = from + i * stride;
           const float mi = a.rows_ml[2 * p], li = a.rows_ml[2 * p + 1];
           l += m > -INFINITY && mi == -INFINITY ? 0.f : li * __builtin_amdgcn_exp2f(mi == -INFINITY ? 0.f : mi - ref);
-          acc += factor(mi - ref) * *reinterpret_cast<const f32x4*>(a.rows_o + p * kD + d);
+          acc += lowered(*reinterpret_cast<const f32x4*>(a.rows_o + p * kD + d), __builtin_amdgcn_exp2f(mi - ref));
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
         *reinterpret_cast<u32x2*>(out + d) =

@@ -336,6 +336,27 @@ def test_shares_of_plans_past_2_to_the_24_tiles(gpu, n):
     assert torch.equal(out.float(), value.repeat_interleave(n).view(-1, 1, 1).expand(-1, 32, 128))
 
 
+def _far_apart(c, b, first, size):
+    """Scores of sequence b's first keys some 600 (log2) below those behind, at values of that size."""
+    c["q"][:, :, 0] = 16.0
+    for j in range(c["lengths"][b]):
+        at = int(c["table"][b, j // c["page"]]), slice(None), j % c["page"]
+        c["kp"][at][:, 0] = 0.0 if j < first else 300.0
+        if j < first:
+            c["vp"][at] = torch.where(c["vp"][at] > 0, size, -size).to(BF16)
+
+
+@pytest.mark.parametrize("lengths,counts,max_new", [([500, 90], [1, 1], 1), ([300, 90], [5, 2], 5), ([4000, 90], [1, 1], 1),
+                                                    ([4000, 90], [5, 2], 5), ([400, 90], [70, 2], None),
+                                                    ([4200, 90], [70, 2], None), ([5000], [37], None)])
+def test_large_values_of_small_probabilities(gpu, lengths, counts, max_new):
+    """Values of 10^36 whose probabilities underflow add nothing, in any form, share or join (sums of 250: below 3e38)."""
+    for first in (1, 130, 250):
+        c = _paged_case(gpu, lengths, counts, 1, 4, 64, seed=first)
+        _far_apart(c, 0, first, 1e36)
+        ref.check(_run_paged(c, gpu, max_new=max_new), *_expect_paged(c), bits=_bits(c, max_new))
+
+
 def test_sequences_of_2_to_the_31_groups_together(gpu):
     """64 sequences of as many tokens as a table can hold, all of them one page, over and over: the mean of equal values.
     (Sums of ones, below 2^24 in a wave: exact.)"""
