@@ -619,7 +619,7 @@ constexpr int kMinTiles = 4;  // a share's tiles, at least: less is a workgroup'
 constexpr int kShareGain = 8;
 constexpr float kGainRows = 4600.f;  // rows for one tile more, for each share
 constexpr int resident(int tile_rows) { return 65536 / tile_rows; }  // workgroups at once
-constexpr float kSlack = 8.f;  // how far (in log2) a score may pass the reference before that moves
+constexpr float kSlack = 8.f;  // how far (in log2) the reference is set above the largest score
 
 // What a sequence is for the rows kernel: its row tiles, the tiles of keys that the last of them sees (the most), and the
 // first.
@@ -1018,10 +1018,11 @@ __global__ void __launch_bounds__(64 * kWaves, 2) rows_kernel(Args a) {
       for (int r = 0; r < 16; ++r) mx = __builtin_elementwise_maximum(mx, s[u][r]);
     return largest_half(mx);
   };
-  // The reference moves only when a score passes it by 2^kSlack: the ratio of the sums does not depend on it.
+  // The reference moves only when a score passes it, to kSlack above that: the ratio of the sums does not depend on it, and
+  // no probability is above one.
   auto refer = [&](float mx) __attribute__((always_inline)) {
-    if (__any(mx > m + kSlack)) {  // wave-uniform
-      const float mn = fmaxf(m, mx);
+    if (__any(mx > m)) {  // wave-uniform
+      const float mn = fmaxf(m, mx + kSlack);
       const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
       m = mn;
       l *= f;

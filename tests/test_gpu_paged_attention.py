@@ -357,6 +357,18 @@ def test_large_values_of_small_probabilities(gpu, lengths, counts, max_new):
         ref.check(_run_paged(c, gpu, max_new=max_new), *_expect_paged(c), bits=_bits(c, max_new))
 
 
+@pytest.mark.parametrize("n,max_new,G", [(1, 1, 4), (6, 6, 4), (80, None, 4), (600, None, 16)])
+def test_a_value_near_the_largest(gpu, n, max_new, G):
+    """Of a score 7 (log2) above the others': its share of the sum, finite as the sum is."""
+    c = _paged_case(gpu, [n + 200, 90], [n, 1], 2, G, 64, seed=n, width=64)
+    c["q"][:], c["kp"][:] = 0, 0
+    c["q"][:, :, 0] = 1.0
+    at = int(c["table"][0, 2]), slice(None), 5
+    c["kp"][at][:, 0] = 55.0
+    c["vp"][at][:, :60] = 2.5e38
+    ref.check(_run_paged(c, gpu, max_new=max_new), *_expect_paged(c), bits=_bits(c, max_new))
+
+
 def test_sequences_of_2_to_the_31_groups_together(gpu):
     """64 sequences of as many tokens as a table can hold, all of them one page, over and over: the mean of equal values.
     (Sums of ones, below 2^24 in a wave: exact.)"""
