@@ -8,6 +8,7 @@
 // maxima are fp32, keys and values bf16 as they lie in memory.
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <type_traits>
 
 #include "skv_common.h"
@@ -1480,8 +1481,11 @@ __global__ void __launch_bounds__(256) rows_join_kernel(Args a, int few_wgs) {
 
 constexpr int64_t kMaxThreads = int64_t{1} << 32;  // of a launch
 
-// The scale's magnitude in units of log2: positive, so that a hidden key's -inf stays one.
-float log2_scale(float scale) { return std::max(std::fabs(scale) * 1.44269504088896340736f, 1.17549435e-38f); }
+// The scale's magnitude in units of log2: positive, so that a hidden key's -inf stays one, and as small as that can be, so
+// that a scale of zero makes 2^-21 of the largest product.
+float log2_scale(float scale) {
+  return std::max(std::fabs(scale) * 1.44269504088896340736f, std::numeric_limits<float>::denorm_min());
+}
 
 bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -1636,7 +1640,7 @@ extern "C" int skv_paged_attn(const uint16_t* q, int64_t q_stride_t, int64_t q_s
                   batch_size, q_heads, kv_heads, max_new, window, pages, width);
     return SKV_EINVAL;
   }
-  if (!std::isfinite(scale)) {
+  if (!std::isfinite(log2_scale(scale))) {
     skv_set_error("%s: scale=%g", what, static_cast<double>(scale));
     return SKV_EINVAL;
   }
@@ -1699,7 +1703,7 @@ extern "C" int skv_packed_attn(const uint16_t* q, int64_t q_stride_t, int64_t q_
                   window);
     return SKV_EINVAL;
   }
-  if (!std::isfinite(scale)) {
+  if (!std::isfinite(log2_scale(scale))) {
     skv_set_error("%s: scale=%g", what, static_cast<double>(scale));
     return SKV_EINVAL;
   }

@@ -369,6 +369,15 @@ def test_a_value_near_the_largest(gpu, n, max_new, G):
     ref.check(_run_paged(c, gpu, max_new=max_new), *_expect_paged(c), bits=_bits(c, max_new))
 
 
+@pytest.mark.parametrize("counts,max_new", [([2, 3], 3), ([70, 40], None)])
+def test_scale_of_zero_at_large_products(gpu, counts, max_new):
+    """The mean of the values, whatever the products of queries and keys are."""
+    c = _paged_case(gpu, [300, 77], counts, 1, 4, 16, seed=4)
+    c["q"][:, :, 0], c["kp"][..., 0] = 1e19, c["kp"][..., 0].sign() * 1e19
+    for scale in (0.0, -0.0, 1e-45):
+        ref.check(_run_paged(c, gpu, max_new=max_new, scale=scale), *_expect_paged(c, scale=0.0), bits=_bits(c, max_new))
+
+
 def test_sequences_of_2_to_the_31_groups_together(gpu):
     """64 sequences of as many tokens as a table can hold, all of them one page, over and over: the mean of equal values.
     (Sums of ones, below 2^24 in a wave: exact.)"""

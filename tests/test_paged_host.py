@@ -267,3 +267,10 @@ def test_more_new_tokens_than_the_host_said(cache):
         _step(cache, 2, [1, 1], max_new=1)
     _step(cache, 40, [1, 39], max_new=1)
     assert cache.lengths.tolist() == [52, 50] and int(cache.lengths.max()) <= cache.get_kv_len()
+
+
+@pytest.mark.parametrize("name,args", [("skv_paged_attn", PAGED), ("skv_packed_attn", PACKED)])
+def test_scales_that_pass_the_largest_number_are_refused(name, args):
+    """As exponents of two: times log2(e)."""
+    for scale in (2.4e38, -3.4e38):
+        _refused(name, args, "scale=", scale=scale)
