@@ -165,14 +165,17 @@ __device__ __forceinline__ void clear_rows(const Args& a, int from, int to, int 
 // V^T P^T, whose first is the lane's 8 tokens of one dim: neither probabilities nor values cross lanes. A probability
 // enters as two bf16 parts (16 significant bits; the matrix cores have the time). 16 keys in a row lie in one page, whose
 // number is a scalar load ahead of theirs. Measured (MI355X, 4 query heads on each of 8 kv heads, with the join): 16
-// sequences of up to 122880 tokens 686 us, 6.2 TB/s where reads reach 6.45; 3 drafted tokens of 6 of up to 30011 in pages
-// of 16 tokens 97 us, 4.4 TB/s (two tiles of rows, two waves a SIMD).
+// sequences of up to 122880 tokens 688 us, 6.2 TB/s where reads reach 6.45; 1 to 5 drafted tokens of 6 of up to 30011 in
+// pages of 16 tokens 98 us, 4.4 TB/s (up to 20 rows: two tiles for every sequence of the call, two waves a SIMD).
 constexpr int kGroup = 32;
 constexpr int kGroupShift = 5;
 constexpr int kMinGroups = 8;  // a chunk's groups, at least
 constexpr int kOutLd = kD + 4;
-// Chunks to aim for: two workgroups for each that the chip holds at once (16 sequences of 65000 keys, 4 query heads on
-// each of 8 kv heads, 768 / 1536 / 2048 chunks: 663 / 667 / 671 us; 24 of 8192 144 / 147 / 152).
+// Chunks to aim for: two workgroups for each that the chip holds at once, since sequences of different lengths end in
+// shorter chunks, and with one each the last of them run alone (4 query heads on each of 8 kv heads, behind a fill of 1 GB,
+// 768 / 1024 / 1536 / 2304 chunks: 16 sequences of 7680 to 122880 keys 944 / 890 / 892 / 886 us, 32 of up to 30000 180 / 172 /
+// 170 / 171, 16 of 65000 725 / 729 / 729 / 736; two tiles, 512 / 768 / 1024 / 1536: 6 of up to 30011 keys 164 / 153 / 156 /
+// 148, 24 of up to 8000 164 / 151 / 156 / 152).
 constexpr int target_chunks(int rows) { return rows <= 16 ? 1536 : 1024; }
 // Groups that a sequence's rows can see (by the table's width and the window) up to which one workgroup of 8 waves takes
 // them all, in one launch: what a CU reads by itself while the chip has room, twice that where sequences and kv heads fill
@@ -1545,6 +1548,8 @@ Plan plan_of(bool paged, int64_t N, int64_t B, int H, int G, int max_new, int64_
     p.rows_grid = items + (p.splits ? 2 * at_once : 0);
     if (p.splits) {
       const int64_t cut = std::min<int64_t>(4 * at_once, items * ((tiles + kMinTiles - 1) / kMinTiles));
+      // (what is cut has more tiles than a share, so that its shares are at most twice the workgroups that the chip holds;
+      // as many again for what the plan rounds: a share without a place would leave its rows)
       p.rows_parts = (cut + H) * tile_rows;
       p.rows_join = std::min<int64_t>(2048, N * G * H);
     }
