@@ -1519,7 +1519,9 @@ Plan plan_of(bool paged, int64_t N, int64_t B, int H, int G, int max_new, int64_
   const int64_t keys = window ? std::min<int64_t>(cap, static_cast<int64_t>(window) + max_new - 1) : cap;
   const bool all_few = paged && static_cast<int64_t>(max_new) * G <= 32;
   // One sequence beside whose rows there are no others has one form, and so have tables of a few tiles: one launch, no join
-  // (up to 25 new tokens of each of 24 sequences of up to 473: 32 -> 25 us). The others': up to 16 rows, one tile.
+  // (up to 25 new tokens of each of 24 sequences of up to 473: 32 -> 25 us). Single tokens and drafts among them then take
+  // bf16 probabilities, as the pieces beside them do: 2^-9 of the values' mean magnitude beside the 2^-9 of the output's own
+  // rounding, where the few-row form has 2^-17. The others': up to 16 rows, one tile.
   if (all_few) p.few_max = max_new;
   else if (paged && B > 1 && cap >= (kMinTiles + kShareGain) * kTile) p.few_max = 16 / G;
   if (p.few_max) {
